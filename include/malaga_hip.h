@@ -59,6 +59,22 @@ typedef struct mlg_model mlg_model;
 typedef struct mlg_batch mlg_batch;
 typedef struct mlg_matrix mlg_matrix;
 
+/* A K/V cache in pages, the caller's memory on the device (mlg_kv_write, mlg_kv_read,
+   mlg_attn_paged).  Each page holds `page` consecutive tokens of one sequence, K and V of every
+   head; a sequence's tokens are the pages that its row of the table lists, in order.  Sequences
+   may list the same page (a shared prefix) as long as none writes to it. */
+typedef struct {
+    uint32_t type;         /* MLG_F16, or MLG_Q8_0: blocks of 32 values of one token and head */
+    int heads;             /* K/V heads */
+    int head_size;         /* 32, 64, 128 or 256 */
+    int page;              /* tokens of a page: 32, 64, 128 or 256 */
+    int pages;             /* pages of the pool */
+    void *pool;            /* pages * mlg_kv_page_bytes(..) bytes, 16-byte aligned */
+    const uint32_t *table; /* [seqs][table_len] page ids, on the device */
+    int seqs;
+    int table_len;         /* page * table_len < 2^31 */
+} mlg_kv_cache;
+
 /* Hyper-parameters: src/config.rs:14-39 (field for field). */
 typedef struct {
     int vocab_size, d_model, encoder_layers, decoder_layers, encoder_heads, decoder_heads;
@@ -228,6 +244,15 @@ void mlg_debug_fail_alloc_after(long n);
    writes it to out when cap holds it.  No counterpart in the reference (the layout is this
    backend's). */
 int64_t mlg_debug_tile_major(uint32_t type, int N, int K, const void *gguf_rows, void *out, int64_t cap);
+/* Test hook, no device used: byte of value (token pos of the sequence, head, dim) of K (which = 0)
+   or V (1) in a page's sequence tile, from the pool's first byte, for page id `id`; q8_0 also the
+   byte of its block's scale (scale_byte, may be NULL; f16: -1).  -1: an argument out of range. */
+int64_t mlg_debug_kv_place(const mlg_kv_cache *c, uint32_t id, int head, int which, int pos, int dim,
+                           int64_t *scale_byte);
+/* Test hook, no device used: the rows and tokens that the kernels take sequence i to have, from
+   arrays on the host: its first row, rows, tokens, and whether it is usable. */
+int mlg_debug_kv_seq(const mlg_kv_cache *c, const uint32_t *row_off, const uint32_t *ctx, int rows, int max_new, int i,
+                     int *first, int *n, int *tokens, int *usable);
 /* Streaming-read ceiling, the reference point of the LM head's roofline (measurement only;
    no counterpart in the reference): `grid` workgroups of 256 threads read every 16-byte word
    of p[0, bytes) once, 8 loads of 16 bytes in flight per thread; mode 0 ordinary loads,
@@ -271,6 +296,56 @@ int mlg_layernorm(const float *x, int rows, int d, const float *gamma, const flo
    32, 64, 128, 256 (else MLG_ERR_UNSUPPORTED); n = lens[row] keys, or *step + 1 without lens. */
 int mlg_attn_decode(const float *q, const void *K, const void *V, int b, int H, int hd, int L, const uint32_t *lens,
                     const uint32_t *step, float *out, void *stream);
+/* ---- a K/V cache in pages: its rows, and attention over it (no counterpart in the reference,
+   whose caches are dense, one length for the whole batch and f16 or f32) ----
+   Bytes of one page, or -1 for a type, head size or page size that is not one of the above.
+   A page is [head][K, V][tile of 32 tokens]; a tile of head size D holds, (t, d) a token of the
+   tile and a dimension (all divisions whole),
+     f16, 64 D bytes: K at element ((d/32*2 + t/4%2)*64 + d/8%4*16 + t/8*4 + t%4)*8 + d%8,
+                      V at element (d/16*64 + t/8*16 + d%16)*8 + t%8;
+     q8_0, 34 D bytes: int8 K at ((d/32*64 + d/8%4*16 + t/8*4 + t%4)*2 + t/4%2)*8 + d%8,
+                      V at ((d/32*64 + t/8*16 + d%16)*2 + d/16%2)*8 + t%8, then at byte
+                      32 D + (d/32*32 + t)*2 the block's f16 scale. */
+int64_t mlg_kv_page_bytes(uint32_t type, int heads, int head_size, int page);
+/* What the next three have in common.  Sequence i's rows are row_off[i] .. row_off[i + 1] - 1 of
+   the row arrays (row_off [seqs + 1], falling nowhere; NULL: max_new rows for every sequence), it
+   may have none, and the cache holds ctx[i] of its tokens (both arrays on the device).  rows: rows
+   that the arrays have; max_new: the most rows of any sequence.  Row arrays are f32, row r at
+   p + r * ld, head h of it at + h * head_size; 16-byte aligned, ld % 4 == 0.  Rows that are no
+   sequence's are neither read nor written.
+   What only the device can see is checked there: a sequence with more tokens than its table row
+   holds, more rows than max_new, falling or too large offsets, and a page id that is not below
+   `pages` are not followed; *bad (a device word, or NULL) is then set to 1, and is left alone
+   otherwise.  Nothing of such a sequence is written; its rows (those below `rows`, at most max_new
+   of them) read and attend as zeros; tokens on such a page are not written, read as zeros, and are
+   no keys.
+   No call allocates, waits or uses memory other than its arguments, so each may be captured and
+   may run beside any other that does not write what it reads.  The stream's device is current.
+   mlg_kv_write: K and V of the rows, each sequence's last tokens (positions ctx - n .. ctx - 1;
+   ctx < n: bad), into the cache; two rows with one place (a page listed twice): which one the
+   cache then holds is not defined.  f16 rounds to nearest even (beyond 65504: inf).  q8_0
+   quantises as mlg_quantize does: d = max |x| / 127, q = round(x / d); a block with inf or NaN
+   reads back as NaN. */
+int mlg_kv_write(const mlg_kv_cache *c, const float *k, int64_t ldk, const float *v, int64_t ldv,
+                 const uint32_t *row_off, const uint32_t *ctx, int rows, int max_new, uint32_t *bad, void *stream);
+/* The reverse: rows of the cache's tokens as f32. */
+int mlg_kv_read(const mlg_kv_cache *c, float *k, int64_t ldk, float *v, int64_t ldv, const uint32_t *row_off,
+                const uint32_t *ctx, int rows, int max_new, uint32_t *bad, void *stream);
+/* out = softmax(scale q K^T) V for each row and each of `heads` query heads (a multiple of the
+   cache's; head h reads K/V head h / (heads / cache heads)).  causal: a row is one of its sequence's
+   last tokens, written before this call, and sees the tokens up to itself: t of n rows the first
+   ctx - n + t + 1 (none where ctx - n + t < 0).  Otherwise every row sees all ctx tokens (cross
+   attention; beams that share a source).  A row that sees no token, or only scores of -inf, is zero.
+   Tokens that a row does not see have no influence, whatever the cache holds there; where V of one
+   that it sees is inf or NaN, the row is not finite in that dimension.  Results are as
+   f32 arithmetic gives them on the cache's values; repeats are equal bit for bit.
+   max_ctx: about the largest ctx, for the plan alone (any value is right; 0: what the table can hold).
+   scratch: mlg_attn_paged_scratch bytes for the same arguments, 16-byte aligned, the call's own
+   until it has run (two captured graphs that may overlap need two). */
+size_t mlg_attn_paged_scratch(const mlg_kv_cache *c, int heads, int rows, int max_new, int max_ctx);
+int mlg_attn_paged(const mlg_kv_cache *c, const float *q, int64_t ldq, int heads, float scale, int causal,
+                   const uint32_t *row_off, const uint32_t *ctx, int rows, int max_new, int max_ctx, float *out,
+                   int64_t ldo, void *scratch, size_t scratch_bytes, uint32_t *bad, void *stream);
 /* argmax_partial (kernels/malaga.cu:247-280): pv/pi [b][parts]. */
 int mlg_argmax_partial(const float *logits, int b, int V, int mask_id, float *pv, uint32_t *pi, int parts,
                        void *stream);

@@ -49,6 +49,14 @@ class ShortlistSpec(C.Structure):
     _fields_ = [("code", C.c_char_p), ("lang_id", C.c_uint32), ("ids", C.POINTER(C.c_uint32)), ("n_ids", C.c_int)]
 
 
+class KvCache(C.Structure):
+    """mlg_kv_cache: a K/V cache in pages (device pointers)."""
+
+    _fields_ = [("type", C.c_uint32), ("heads", C.c_int), ("head_size", C.c_int), ("page", C.c_int),
+                ("pages", C.c_int), ("pool", C.c_void_p), ("table", C.c_void_p), ("seqs", C.c_int),
+                ("table_len", C.c_int)]
+
+
 TENSOR_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_char_p, C.c_int64, C.POINTER(C.c_float))
 # mlg_beam_decode_fn(user, step, rows, reorder, next, vals, idx)
 BEAM_DECODE_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32),
@@ -126,6 +134,15 @@ SIGNATURES = {
     "mlg_residual_ln": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, _P, C.c_float, _P, _P]),
     "mlg_layernorm": (C.c_int, [_P, C.c_int, C.c_int, _P, _P, C.c_float, _P, _P]),
     "mlg_attn_decode": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P]),
+    "mlg_kv_page_bytes": (C.c_int64, [C.c_uint32, C.c_int, C.c_int, C.c_int]),
+    "mlg_kv_write": (C.c_int, [C.POINTER(KvCache), _P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int, C.c_int, _P, _P]),
+    "mlg_kv_read": (C.c_int, [C.POINTER(KvCache), _P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int, C.c_int, _P, _P]),
+    "mlg_attn_paged_scratch": (C.c_size_t, [C.POINTER(KvCache), C.c_int, C.c_int, C.c_int, C.c_int]),
+    "mlg_attn_paged": (C.c_int, [C.POINTER(KvCache), _P, C.c_int64, C.c_int, C.c_float, C.c_int, _P, _P, C.c_int,
+                                 C.c_int, C.c_int, _P, C.c_int64, _P, C.c_size_t, _P, _P]),
+    "mlg_debug_kv_place": (C.c_int64, [C.POINTER(KvCache), C.c_uint32, C.c_int, C.c_int, C.c_int, C.c_int,
+                                       C.POINTER(C.c_int64)]),
+    "mlg_debug_kv_seq": (C.c_int, [C.POINTER(KvCache), _P, _P, C.c_int, C.c_int, C.c_int, _intp, _intp, _intp, _intp]),
     "mlg_argmax_partial": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, _P, _P, C.c_int, _P]),
     "mlg_greedy_finalize": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, _P, _P, C.c_int, _P, C.c_uint32, C.c_uint32,
                                       _P]),

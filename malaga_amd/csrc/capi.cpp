@@ -3,6 +3,7 @@
 // thread-local message.
 #include "../../include/malaga_hip.h"
 
+#include <cmath>
 #include <cstring>
 #include <initializer_list>
 #include <memory>
@@ -10,6 +11,7 @@
 
 #include "beam.hpp"
 #include "convert.hpp"
+#include "paged_kv.hpp"
 #include "quant.hpp"
 #include "runtime.hpp"
 #include "server.hpp"
@@ -137,6 +139,56 @@ int write_rows(const std::vector<std::vector<uint32_t>> &rows, uint32_t *out, in
 }
 
 hipStream_t as_stream(void *s) { return static_cast<hipStream_t>(s); }
+
+bool kv_size_ok(int hd, int page) {
+    return (hd == 32 || hd == 64 || hd == 128 || hd == 256) && (page == 32 || page == 64 || page == 128 || page == 256);
+}
+
+mlg::KvPool kv_pool(const mlg_kv_cache *c) {
+    int shift = 5;
+    while ((1 << shift) < c->page) ++shift;
+    return {static_cast<uint8_t *>(c->pool), c->table, c->seqs, c->table_len, c->heads, c->pages, shift};
+}
+
+int kv_max_ctx(const mlg_kv_cache *c, int max_ctx) {
+    const int64_t most = int64_t(c->page) * c->table_len;
+    return int(max_ctx > 0 && max_ctx < most ? max_ctx : most);
+}
+
+// What the calls on a paged cache check alike: the cache, the two row arrays and their strides.
+int check_kv(const mlg_kv_cache *c, std::initializer_list<const void *> arrays, std::initializer_list<int64_t> strides,
+             int heads, const uint32_t *row_off, const uint32_t *ctx, int rows, int max_new, hipStream_t st,
+             const char *what) {
+    const std::string w(what);
+    if (!c || !c->pool || !c->table || !ctx || c->heads < 1 || c->pages < 1 || c->seqs < 0 || c->table_len < 1 ||
+        rows < 0 || max_new < 1)
+        return set_err(MLG_ERR_INVALID, w + ": bad argument");
+    if (c->type != MLG_F16 && c->type != MLG_Q8_0) return set_err(MLG_ERR_UNSUPPORTED, w + ": cache type (f16, q8_0)");
+    if (!kv_size_ok(c->head_size, c->page))
+        return set_err(MLG_ERR_UNSUPPORTED, w + ": head size and page of 32, 64, 128 or 256");
+    if (int64_t(c->page) * c->table_len > 0x7fffffff)
+        return set_err(MLG_ERR_INVALID, w + ": more than 2^31 - 1 tokens in a table row");
+    if (int64_t(heads) * c->head_size > 0x7fffffff) return set_err(MLG_ERR_INVALID, w + ": too many heads");
+    if (!row_off && int64_t(c->seqs) * max_new > rows)
+        return set_err(MLG_ERR_INVALID, w + ": fewer rows than max_new for every sequence");
+    for (const void *p : arrays)
+        if (!p) return set_err(MLG_ERR_INVALID, w + ": null argument");
+    for (int64_t ld : strides)
+        if (ld < int64_t(heads) * c->head_size || ld % 4)
+            return set_err(MLG_ERR_INVALID, w + ": row stride below heads * head_size, or not a multiple of 4");
+    if (!aligned16(arrays) || !aligned16({c->pool}))
+        return set_err(MLG_ERR_INVALID, w + ": rows and pool must be 16-byte aligned");
+    // launches go to the current device: a stream of another is refused
+    if (st && c->seqs > 0 && rows > 0) {
+        int cur = 0;
+        hipDevice_t dev = 0;
+        hipError_t e = hipGetDevice(&cur);
+        if (e == hipSuccess) e = hipStreamGetDevice(st, &dev);
+        if (e != hipSuccess) return hip_status(e, what);
+        if (int(dev) != cur) return set_err(MLG_ERR_INVALID, w + ": the stream's device is not current");
+    }
+    return MLG_OK;
+}
 
 }  // namespace
 
@@ -676,6 +728,83 @@ int mlg_attn_decode(const float *q, const void *K, const void *V, int b, int H, 
     return hip_status(mlg::attn_decode(q, static_cast<const __half *>(K), static_cast<const __half *>(V), b, H, hd, L,
                                        lens, lens ? nullptr : step, out, as_stream(stream)),
                       "attn_decode");
+}
+
+int64_t mlg_kv_page_bytes(uint32_t type, int heads, int head_size, int page) {
+    const bool ok = (type == MLG_F16 || type == MLG_Q8_0) && heads > 0 && kv_size_ok(head_size, page);
+    return ok ? int64_t(heads) * 2 * (page / mlg::kKvTile) * mlg::kv_tile_bytes(type == MLG_Q8_0, head_size) : -1;
+}
+
+int mlg_kv_write(const mlg_kv_cache *c, const float *k, int64_t ldk, const float *v, int64_t ldv,
+                 const uint32_t *row_off, const uint32_t *ctx, int rows, int max_new, uint32_t *bad, void *stream) {
+    const int e = check_kv(c, {k, v}, {ldk, ldv}, c ? c->heads : 0, row_off, ctx, rows, max_new, as_stream(stream),
+                           "kv_write");
+    if (e != MLG_OK) return e;
+    return hip_status(mlg::kv_write(kv_pool(c), c->type == MLG_Q8_0, c->head_size, k, size_t(ldk), v, size_t(ldv),
+                                    {row_off, ctx, rows, max_new, bad}, as_stream(stream)),
+                      "kv_write");
+}
+
+int mlg_kv_read(const mlg_kv_cache *c, float *k, int64_t ldk, float *v, int64_t ldv, const uint32_t *row_off,
+                const uint32_t *ctx, int rows, int max_new, uint32_t *bad, void *stream) {
+    const int e = check_kv(c, {k, v}, {ldk, ldv}, c ? c->heads : 0, row_off, ctx, rows, max_new, as_stream(stream),
+                           "kv_read");
+    if (e != MLG_OK) return e;
+    return hip_status(mlg::kv_read(kv_pool(c), c->type == MLG_Q8_0, c->head_size, k, size_t(ldk), v, size_t(ldv),
+                                   {row_off, ctx, rows, max_new, bad}, as_stream(stream)),
+                      "kv_read");
+}
+
+size_t mlg_attn_paged_scratch(const mlg_kv_cache *c, int heads, int rows, int max_new, int max_ctx) {
+    if (!c || mlg_kv_page_bytes(c->type, c->heads, c->head_size, c->page) < 0 || heads < 1 || heads % c->heads ||
+        rows < 1 || max_new < 1 || c->seqs < 1 || c->table_len < 1)
+        return 0;
+    return mlg::attn_paged_scratch(kv_pool(c), c->head_size, heads, rows, max_new, kv_max_ctx(c, max_ctx));
+}
+
+int mlg_attn_paged(const mlg_kv_cache *c, const float *q, int64_t ldq, int heads, float scale, int causal,
+                   const uint32_t *row_off, const uint32_t *ctx, int rows, int max_new, int max_ctx, float *out,
+                   int64_t ldo, void *scratch, size_t scratch_bytes, uint32_t *bad, void *stream) {
+    if (!c || heads < 1 || c->heads < 1 || heads % c->heads || !std::isfinite(scale) || max_ctx < 0)
+        return set_err(MLG_ERR_INVALID, "attn_paged: bad argument");
+    const int e = check_kv(c, {q, out}, {ldq, ldo}, heads, row_off, ctx, rows, max_new, as_stream(stream),
+                           "attn_paged");
+    if (e != MLG_OK) return e;
+    const size_t need = mlg_attn_paged_scratch(c, heads, rows, max_new, max_ctx);
+    if (need && (!scratch || scratch_bytes < need || !aligned16({scratch})))
+        return set_err(MLG_ERR_INVALID, "attn_paged: " + std::to_string(need) + " bytes of 16-byte aligned scratch needed");
+    return hip_status(mlg::attn_paged(kv_pool(c), c->type == MLG_Q8_0, c->head_size,
+                                      {q, out, size_t(ldq), size_t(ldo), heads, causal != 0, scale,
+                                       static_cast<float *>(scratch)},
+                                      {row_off, ctx, rows, max_new, bad}, kv_max_ctx(c, max_ctx), as_stream(stream)),
+                      "attn_paged");
+}
+
+int64_t mlg_debug_kv_place(const mlg_kv_cache *c, uint32_t id, int head, int which, int pos, int dim,
+                           int64_t *scale_byte) {
+    if (scale_byte) *scale_byte = -1;
+    if (!c || mlg_kv_page_bytes(c->type, c->heads, c->head_size, c->page) < 0 || id >= uint32_t(c->pages) || head < 0 ||
+        head >= c->heads || which < 0 || which > 1 || pos < 0 || dim < 0 || dim >= c->head_size)
+        return -1;
+    const bool q8 = c->type == MLG_Q8_0;
+    const int t = pos % mlg::kKvTile;
+    const int64_t tile = int64_t(kv_pool(c).tile_at(id, head, which, pos, mlg::kv_tile_bytes(q8, c->head_size)));
+    const int e = which ? mlg::kv_v_elem(q8, t, dim) : mlg::kv_k_elem(q8, t, dim);
+    if (q8 && scale_byte) *scale_byte = tile + mlg::kv_scale_byte(c->head_size, t, dim / 32);
+    return tile + (q8 ? e : 2 * e);
+}
+
+int mlg_debug_kv_seq(const mlg_kv_cache *c, const uint32_t *row_off, const uint32_t *ctx, int rows, int max_new, int i,
+                     int *first, int *n, int *tokens, int *usable) {
+    if (!c || mlg_kv_page_bytes(c->type, c->heads, c->head_size, c->page) < 0 || !ctx || i < 0 || i >= c->seqs ||
+        max_new < 1 || !first || !n || !tokens || !usable)
+        return set_err(MLG_ERR_INVALID, "bad argument");
+    const mlg::KvSeq s = mlg::kv_seq(kv_pool(c), {row_off, ctx, rows, max_new, nullptr}, i);
+    *first = s.r0;
+    *n = s.n;
+    *tokens = s.ctx;
+    *usable = s.ok;
+    return MLG_OK;
 }
 
 int mlg_argmax_partial(const float *logits, int b, int V, int mask_id, float *pv, uint32_t *pi, int parts,
