@@ -9,8 +9,8 @@
 //
 // Results are as exact as f32 arithmetic: K and V are exact operands (f16, or the whole numbers of a
 // q8_0 block, whose scales are applied in f32), and q and p enter as two f16 each (hi = f16(x), lo =
-// f16(x - hi): 22 bits), which doubles the matrix work. q is scaled by a power of two per row and p by
-// 2^15 (its maximum is 1) so that what lo loses below f16's range is 2^-29 of the largest value. Sums
+// f16(x - hi): 22 bits), which doubles the matrix work. q is scaled by a power of two per row, and p's
+// largest held between 2^7 and 2^15, so that what lo loses below f16's range is 2^-31 of the largest value. Sums
 // are f32.
 #include <type_traits>
 
@@ -22,7 +22,9 @@ namespace {
 
 constexpr int kRows = 16;        // rows of a query tile (columns of the matrix products)
 constexpr int kWaves = 4;        // waves of a workgroup
-constexpr float kPShift = 15.f;  // p is held times 2^15
+// p = 2^(s - m): m is the running maximum of the scores (log2 units) less kPShift, and follows a larger
+// one only when it is kPSlack or more behind, which after the first tiles is rare: p stays below 2^15.
+constexpr float kPShift = 7.f, kPSlack = 8.f;
 
 // Partial result of a split: [m, l, -, -, out of HD dims] of one row, f32, as a Tile holds them.
 constexpr int kPartHead = 4;
@@ -150,6 +152,8 @@ struct Frags {
 // 2^-22 on average; rounding lo to nearest measured 4 more operations per pair of values).
 __device__ __forceinline__ void split8(const float (&p)[8], h8_t &hi, h8_t &lo) {
     uint32_t h[4], l[4];
+    float minus = -1.f;  // not a constant to the compiler, which keeps x - hi one operation (v_fma_mix)
+    asm("" : "+s"(minus));
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         // p as finished f32 values: hi's and lo's uses of a product are otherwise rounded apart
@@ -157,7 +161,7 @@ __device__ __forceinline__ void split8(const float (&p)[8], h8_t &hi, h8_t &lo) 
         asm("" : "+v"(x), "+v"(y));
         const h2_t t = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x, y));
         h[n] = __builtin_bit_cast(uint32_t, t);
-        l[n] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(float(t[0]), -1.f, x), fmaf(float(t[1]), -1.f, y)));
+        l[n] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(float(t[0]), minus, x), fmaf(float(t[1]), minus, y)));
     }
     hi = as_h8(make_uint4(h[0], h[1], h[2], h[3]));
     lo = as_h8(make_uint4(l[0], l[1], l[2], l[3]));
@@ -236,17 +240,23 @@ struct Tile {
         for (int n = 0; n < 8; ++n) s[n] = acc[n >> 2][n & 3];
     }
 
-    // s becomes p (times 2^15); m, l and out follow a larger maximum.
-    __device__ __forceinline__ void softmax(float (&s)[8]) {
-        float t = vmax3(vmax3(s[0], s[1], s[2]), vmax3(s[3], s[4], s[5]), vmax(s[6], s[7]));
-        t = fmaf(rows_max(t), qf, -kPShift);
-        if (__any(t > m)) {  // wave-uniform
-            const float mn = fmaxf(m, t), al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            l *= al;
+    // The largest score of the lane's row in a tile, as m holds it.
+    __device__ __forceinline__ float top(const float (&s)[8]) const {
+        const float t = vmax3(vmax3(s[0], s[1], s[2]), vmax3(s[3], s[4], s[5]), vmax(s[6], s[7]));
+        return fmaf(rows_max(t), qf, -kPShift);
+    }
+    // Whether it takes a row's p past 2^15.
+    __device__ __forceinline__ bool behind(float t) const { return t > m + kPSlack; }
+    // m, l and out follow it.
+    __device__ __forceinline__ void follow(float t) {
+        const float mn = fmaxf(m, t), al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= al;
 #pragma unroll
-            for (int u = 0; u < NU; ++u) o[u] *= al;
-            m = mn;
-        }
+        for (int u = 0; u < NU; ++u) o[u] *= al;
+        m = mn;
+    }
+    // s becomes p.
+    __device__ __forceinline__ void probs(float (&s)[8]) {
         const float base = m == -INFINITY ? 0.f : m;  // nothing seen: every score is -inf
 #pragma unroll
         for (int n = 0; n < 8; ++n) s[n] = __builtin_amdgcn_exp2f(fmaf(s[n], qf, -base));
@@ -389,157 +399,48 @@ __device__ __forceinline__ void put_row(const KvAttn &a, const Work &w, int spli
     }
 }
 
-// ---- few rows to a K/V head: each wave reads its own tiles straight into registers ----
-template <int HD, bool Q8>
-__global__ __launch_bounds__(256, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) void k_attn_rows(KvPool pool, KvAttn a, KvRows r,
-                                                                                     int group, int splits) {
-    constexpr int TB = kv_tile_bytes(Q8, HD), NU = HD / 16;
-    __shared__ float sm[kWaves][kRows], sl[kWaves][kRows];
-    __shared__ f4_t so[kWaves][NU][64];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t b = blockIdx.x;
-    Work job;
-    job.group = group;
-    job.split = int(b % uint32_t(splits));
-    b /= uint32_t(splits);
-    job.head = int(b % uint32_t(pool.heads));
-    job.i = int(b / uint32_t(pool.heads));
-    const KvSeq s = job.s = kv_seq(pool, r, job.i);
-    if (!s.ok && r.bad && threadIdx.x == 0) *r.bad = 1u;
-    const int rows = s.n * group;
-    if (rows == 0 || rows > kRows) return;  // more: k_attn_chunk's
-    // this lane's row, and the tokens that it and the tile's first and last row see
-    const int row = min(lane & 15, rows - 1);
-    const int least = job.sees(a, 0), most = job.sees(a, rows - 1);
-    const bool have = (lane & 15) < rows;
-    Tile<HD, Q8> t;
-    t.load_q(have ? a.q + job.qrow(row) * a.ldq + size_t(job.qhead(row)) * HD : nullptr, a.scale, lane);
-    t.vis = job.sees(a, row);
-    const int tiles = (most + kKvTile - 1) / kKvTile, per = (tiles + splits - 1) / splits;
-    const int end = min(tiles, (job.split + 1) * per);
-    const uint32_t *table = pool.table + size_t(job.i) * size_t(pool.table_len);
-    // K of the next tile is asked for once this one's is used, V likewise: one of them is always on its way
-    RawTile<HD, Q8> kr, vr;
-    auto page_of = [&](int kt) { return kt < end ? table[kt * kKvTile >> pool.shift] : 0xffffffffu; };
-    auto load = [&](RawTile<HD, Q8> &x, int which, uint32_t page, int kt) __attribute__((always_inline)) {
-        if (page < uint32_t(pool.pages))
-            x.load(pool.pool + pool.tile_at(page, job.head, which, kt * kKvTile, TB), lane);
-    };
-    int kt = job.split * per + w;
-    bool odd = false;
-    uint32_t page = page_of(kt), next = page_of(kt + kWaves);
-    load(kr, 0, page, kt);
-    load(vr, 1, page, kt);
-    auto step = [&](auto masked) __attribute__((always_inline)) {
-        constexpr bool kMasked = decltype(masked)::value;
-        const int tok0 = kt * kKvTile;
-        const bool there = page < uint32_t(pool.pages);
-        float p[8];
-        Frags<HD, Q8> f;
-        if (there) {
-            f.from(kr);
-            t.scores(f, p);
-        } else if (r.bad && lane == 0) {  // its tokens are not there
-            *r.bad = 1u;
-        }
-        load(kr, 0, next, kt + kWaves);
-        if (there) {
-            if constexpr (kMasked) t.hide(p, tok0);
-            t.softmax(p);
-            f.from(vr);
-        }
-        load(vr, 1, next, kt + kWaves);
-        if (there) {
-            if constexpr (kMasked) odd |= f.cut(s.ctx - tok0 - 8 * (lane >> 4));
-            t.template values<kMasked>(f, p);
-        }
-        page = next;
-        next = page_of(kt + 2 * kWaves);
-    };
-    const int whole = min(end, least / kKvTile);
-    for (; kt < whole; kt += kWaves) step(std::false_type{});
-    const int masked0 = kt;
-    for (; kt < end; kt += kWaves) step(std::true_type{});
-    if (__any(odd))  // wave-uniform
-        for (kt = masked0; kt < end; kt += kWaves)
-            if (const uint32_t id = page_of(kt); id < uint32_t(pool.pages))
-                t.not_finite(pool.pool + pool.tile_at(id, job.head, 1, kt * kKvTile, TB), kt * kKvTile, s.ctx);
-    // the waves' results meet in LDS
-    const float lw = t.finish();
-    if (lane < kRows) {
-        sm[w][lane] = t.m;
-        sl[w][lane] = lw;
-    }
-#pragma unroll
-    for (int u = 0; u < NU; ++u) so[w][u][lane] = t.o[u];
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, f[kWaves];
-    const int lr = lane & 15;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) m = fmaxf(m, sm[k][lr]);
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-        // a wave without tokens adds nothing, whatever its zeros would be multiplied by
-        f[k] = sl[k][lr] == 0.f ? 0.f : sm[k][lr] == m ? 1.f : __builtin_amdgcn_exp2f(sm[k][lr] - m);
-        l += sl[k][lr] == 0.f ? 0.f : f[k] * sl[k][lr];
-    }
-    if (!have) return;
-    for (int u = w; u < NU; u += kWaves) {
-        f4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k)
-            if (sl[k][lr] != 0.f) o += so[k][u][lane] * f[k];
-        put_row<HD>(a, job, splits, row, u, lane, o, m, l);
-    }
-}
-
-// ---- many rows to a K/V head: the workgroup's waves share the tiles through LDS ----
-// Eight waves: four groups of QT tiles of rows, twice, one for each of the two tiles of tokens that a
-// stage holds (four waves alone left the SIMDs with two waves each, and neither the matrix unit nor
-// the VALU busy). A stage is fetched into registers while the one before it is worked on, then
-// (q8_0: as f16) put into the other half of LDS: one barrier a stage, and each line of the cache is
-// read once for 64 QT rows. The two halves' results meet in LDS at the end.
-template <int HD, bool Q8>
-struct Chunk {
-    static constexpr int QT = HD <= 128 ? 2 : 1, ST = 2, kWavesWg = 8;
-    static constexpr int kRowsWg = 4 * QT * kRows;
-    static constexpr int NU = HD / 16, NC = HD / 32;
-    static constexpr int kFragBytes = NU * 1024, kScaleBytes = Q8 ? NC * 64 : 0;
-    static constexpr int kTileLds = kFragBytes + kScaleBytes;  // of K or V
-    static_assert(4 * QT * NU * 1024 <= 2 * ST * 2 * kTileLds, "half of the waves' out fits the stages' LDS");
+// RG groups of QT tiles of rows, by TG waves each that take every TG-th tile of tokens. Every wave
+// reads its tiles straight into the registers that the matrix products take them from: K of the next
+// tile is asked for once this one's is used, V likewise, so that one of them is always on its way.
+// Waves of other rows read the same lines at about the same time, out of L1 and L2 (a stage through
+// LDS that eight waves shared measured slower: 298 to 376 us against the 4001-token chunk's figure
+// below, for its barriers and because a stage is worked on in less time than the next takes to come).
+// SKIP: sequences of up to that many rows are another launch's; LIMIT: and those of more.
+template <int HD, bool Q8, int QT, int RG, int TG>
+struct Shape {
+    static constexpr int kRowsWg = RG * QT * kRows, kThreads = 64 * RG * TG;
+    // waves of a SIMD: what the registers of a wave leave room for
+    static constexpr int kWavesSimd = QT == 1 ? (HD <= 64 ? 3 : HD <= 128 ? 2 : 1) : (HD <= 64 ? 3 : 2);
 };
 
-template <int HD, bool Q8>
-__global__ __launch_bounds__(512, HD <= 64 ? 4 : 2) void k_attn_chunk(KvPool pool, KvAttn a, KvRows r, int group,
-                                                                      int row_tiles, int splits, int skip) {
-    typedef Chunk<HD, Q8> C;
-    constexpr int TB = kv_tile_bytes(Q8, HD), NU = HD / 16, QT = C::QT, ST = C::ST;
-    __shared__ uint8_t lds[2][ST][2][C::kTileLds] __attribute__((aligned(16)));
-    __shared__ float sml[2][4][QT][kRows];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = w & 3, kg = w >> 2;
+template <int HD, bool Q8, int QT, int RG, int TG>
+__global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSimd)) void k_attn(
+    KvPool pool, KvAttn a, KvRows r, int group, int row_tiles, int splits, int skip, int limit) {
+    typedef Shape<HD, Q8, QT, RG, TG> S;
+    constexpr int TB = kv_tile_bytes(Q8, HD), NU = HD / 16;
+    __shared__ float sm[TG][RG][QT][kRows], sl[TG][RG][QT][kRows];
+    __shared__ f4_t so[TG][RG][QT][NU][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = w % RG, tg = w / RG;
     uint32_t b = blockIdx.x;
     Work job;
     job.group = group;
     job.split = int(b % uint32_t(splits));
     b /= uint32_t(splits);
     // A K/V head's workgroups are as many apart as there are heads (with 8 or 16 of them all on one of
-    // the 8 XCDs, whose L2 then reads the head's tiles once); the longest row tiles come first, and
-    // every other 256 workgroups in reverse, so that a CU's long ones meet short ones.
+    // the 8 XCDs, whose L2 then reads the head's tiles once); the longest row tiles come first, so that
+    // the short ones fill what is left at the end.
     const uint32_t pairs = uint32_t(pool.seqs) * uint32_t(pool.heads), pair = b % pairs;
-    int rank = int(b / pairs);
-    const int turn = max(1, int(256u / pairs)), fold = rank / turn;
-    if ((fold & 1) && (fold + 1) * turn <= row_tiles) rank = fold * turn + (turn - 1 - rank % turn);
-    const int rt = row_tiles - 1 - rank;
+    const int rt = row_tiles - 1 - int(b / pairs);
     job.head = int(pair % uint32_t(pool.heads));
     job.i = int(pair / uint32_t(pool.heads));
     const KvSeq s = job.s = kv_seq(pool, r, job.i);
     if (!s.ok && r.bad && threadIdx.x == 0) *r.bad = 1u;
-    const int rows = s.n * group, first = rt * C::kRowsWg;
-    if (first >= rows || rows <= skip) return;  // skip: k_attn_rows' sequences
-    const int wg_most = job.sees(a, min(first + C::kRowsWg, rows) - 1);
+    const int rows = s.n * group, first = rt * S::kRowsWg;
+    if (first >= rows || rows <= skip || rows > limit) return;
     const int row0 = first + rg * QT * kRows;  // the wave's first row
     const bool busy = row0 < rows;
-    const int most = job.sees(a, min(row0 + QT * kRows, rows) - 1);
+    // what the wave's first and last row see
+    const int least = job.sees(a, min(row0, rows - 1)), most = busy ? job.sees(a, min(row0 + QT * kRows, rows) - 1) : 0;
     Tile<HD, Q8> t[QT];
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
@@ -547,155 +448,108 @@ __global__ __launch_bounds__(512, HD <= 64 ? 4 : 2) void k_attn_chunk(KvPool poo
         t[j].load_q(mine < rows ? a.q + job.qrow(row) * a.ldq + size_t(job.qhead(row)) * HD : nullptr, a.scale, lane);
         t[j].vis = job.sees(a, row);
     }
-    const int tiles = (wg_most + kKvTile - 1) / kKvTile;
-    const int per = ((tiles + splits - 1) / splits + ST - 1) / ST * ST;
-    const int begin = job.split * per, end = min(tiles, begin + per);
+    // the split's tiles: the same for all of a workgroup's rows
+    const int all = (job.sees(a, min(first + S::kRowsWg, rows) - 1) + kKvTile - 1) / kKvTile;
+    const int per = (all + splits - 1) / splits;
+    const int end = min((most + kKvTile - 1) / kKvTile, (job.split + 1) * per);
     const uint32_t *table = pool.table + size_t(job.i) * size_t(pool.table_len);
-
-    // a thread's share of a stage: 16-byte pieces of the tiles' K and V, and of q8_0's scales
-    constexpr int NP = Q8 ? HD / 32 : HD / 16;  // 1 KB pieces of a tile
-    constexpr int ALL = ST * 2 * NP, NPER = ALL > C::kWavesWg ? ALL / C::kWavesWg : 1;  // pieces; of a wave
-    static_assert(ALL <= C::kWavesWg || ALL % C::kWavesWg == 0, "pieces to waves");
-    constexpr int NS = C::NC * 4;  // 16-byte pieces of a tile's scales
-    u4_t raw[NPER], rsc = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int n = 0; n < NPER; ++n) raw[n] = rsc;
-    uint32_t pages[ST], coming[ST];
-    auto pages_of = [&](int kt, uint32_t (&p)[ST]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < ST; ++j) p[j] = kt + j < end ? table[(kt + j) * kKvTile >> pool.shift] : 0xffffffffu;
+    RawTile<HD, Q8> kr, vr;
+    auto page_of = [&](int kt) __attribute__((always_inline)) {
+        return kt < end ? table[kt * kKvTile >> pool.shift] : 0xffffffffu;
     };
-    auto fetch = [&](int kt, const uint32_t (&p)[ST]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < NPER; ++n) {
-            const int pc = w * NPER + n, j = pc / (2 * NP), which = pc / NP % 2, q = pc % NP;
-            const uint32_t page = j ? p[1] : p[0];
-            if (pc < ALL && page < uint32_t(pool.pages))
-                raw[n] = *reinterpret_cast<const u4_t *>(
-                    pool.pool + pool.tile_at(page, job.head, which, (kt + j) * kKvTile, TB) + (q * 64 + lane) * 16);
-        }
-        if constexpr (Q8) {
-            const int pc = int(threadIdx.x), j = pc / (2 * NS), which = pc / NS % 2, q = pc % NS;
-            const uint32_t page = j ? p[1] : p[0];
-            if (pc < ST * 2 * NS && page < uint32_t(pool.pages))
-                rsc = *reinterpret_cast<const u4_t *>(
-                    pool.pool + pool.tile_at(page, job.head, which, (kt + j) * kKvTile, TB) + 32 * HD + q * 16);
-        }
+    auto load = [&](RawTile<HD, Q8> &x, int which, uint32_t page, int kt) __attribute__((always_inline)) {
+        if (page < uint32_t(pool.pages))
+            x.load(pool.pool + pool.tile_at(page, job.head, which, kt * kKvTile, TB), lane);
     };
-    auto keep = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < NPER; ++n) {
-            const int pc = w * NPER + n, j = pc / (2 * NP), which = pc / NP % 2, q = pc % NP;
-            if (pc >= ALL) continue;
-            uint8_t *at = lds[buf][j][which];
-            if constexpr (Q8) {
-                *reinterpret_cast<h8_t *>(at + ((2 * q) * 64 + lane) * 16) = i8_to_h8(raw[n][0], raw[n][1]);
-                *reinterpret_cast<h8_t *>(at + ((2 * q + 1) * 64 + lane) * 16) = i8_to_h8(raw[n][2], raw[n][3]);
-            } else {
-                *reinterpret_cast<u4_t *>(at + (q * 64 + lane) * 16) = raw[n];
-            }
-        }
-        if constexpr (Q8) {
-            const int pc = int(threadIdx.x), j = pc / (2 * NS), which = pc / NS % 2, q = pc % NS;
-            if (pc < ST * 2 * NS) *reinterpret_cast<u4_t *>(lds[buf][j][which] + C::kFragBytes + q * 16) = rsc;
-        }
-    };
-    auto read = [&](Frags<HD, Q8> &f, const uint8_t *at) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < NU; ++u) f.a[u] = *reinterpret_cast<const h8_t *>(at + (u * 64 + lane) * 16);
-        if constexpr (Q8) {
-#pragma unroll
-            for (int c = 0; c < C::NC; ++c)
-                f.d[c] = *reinterpret_cast<const uint4 *>(at + C::kFragBytes + c * 64 + (lane >> 4) * 16);
-        }
-    };
-
-    if (begin < end) {
-        pages_of(begin, pages);
-        fetch(begin, pages);
-        pages_of(begin + ST, coming);
-        keep(0);
-    }
-    int buf = 0, kt = begin;
+    int kt = job.split * per + tg;
     bool odd = false;
-    auto stage = [&](auto masked) __attribute__((always_inline)) {
+    uint32_t page = page_of(kt), next = page_of(kt + TG);
+    load(kr, 0, page, kt);
+    load(vr, 1, page, kt);
+    auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
-        __syncthreads();  // this stage is in LDS, and the other half is no longer read
-        if (kt + ST < end) fetch(kt + ST, coming);
-        const int tok0 = (kt + kg) * kKvTile;
-        const uint32_t page = kg ? pages[1] : pages[0];
+        const int tok0 = kt * kKvTile;
         const bool there = page < uint32_t(pool.pages);
-        if (!there && kt + kg < end && r.bad && lane == 0) *r.bad = 1u;  // its tokens are not there
-        if (busy && there && (!kMasked || tok0 < most)) {
-            float p[QT][8];
-            Frags<HD, Q8> f;
-            read(f, lds[buf][kg][0]);
+        float p[QT][8];
+        Frags<HD, Q8> f;
+        if (there) {
+            f.from(kr);
 #pragma unroll
             for (int q = 0; q < QT; ++q) t[q].scores(f, p[q]);
-            if constexpr (kMasked) {
+        } else if (r.bad && lane == 0) {  // its tokens are not there
+            *r.bad = 1u;
+        }
+        load(kr, 0, next, kt + TG);
+        if (there) {
+            float top[QT];
+            bool behind = false;
 #pragma unroll
-                for (int q = 0; q < QT; ++q) t[q].hide(p[q], tok0);
+            for (int q = 0; q < QT; ++q) {
+                if constexpr (kMasked) t[q].hide(p[q], tok0);
+                top[q] = t[q].top(p[q]);
+                behind |= t[q].behind(top[q]);
             }
+            if (__any(behind)) {  // wave-uniform
 #pragma unroll
-            for (int q = 0; q < QT; ++q) t[q].softmax(p[q]);
-            read(f, lds[buf][kg][1]);
+                for (int q = 0; q < QT; ++q) t[q].follow(top[q]);
+            }
+            f.from(vr);
+        }
+        load(vr, 1, next, kt + TG);
+        if (there) {
             if constexpr (kMasked) odd |= f.cut(s.ctx - tok0 - 8 * (lane >> 4));
 #pragma unroll
-            for (int q = 0; q < QT; ++q) t[q].template values<kMasked>(f, p[q]);
+            for (int q = 0; q < QT; ++q) {
+                t[q].probs(p[q]);
+                t[q].template values<kMasked>(f, p[q]);
+            }
         }
-        if (kt + ST < end) keep(buf ^ 1);
-#pragma unroll
-        for (int j = 0; j < ST; ++j) pages[j] = coming[j];
-        pages_of(kt + 2 * ST, coming);
-        buf ^= 1;
+        page = next;
+        next = page_of(kt + 2 * TG);
     };
-    // the same for every wave: stages that the workgroup's first row sees whole, then the others
-    const int whole = min(end, job.sees(a, first) / kKvTile) - (ST - 1);
-    for (; kt < whole; kt += ST) stage(std::false_type{});
+    const int whole = min(end, least / kKvTile);
+    for (; kt < whole; kt += TG) step(std::false_type{});
     const int masked0 = kt;
-    for (; kt < end; kt += ST) stage(std::true_type{});
+    for (; kt < end; kt += TG) step(std::true_type{});
     if (__any(odd))  // wave-uniform
-        for (kt = masked0 + kg; kt < end; kt += ST)
-            if (const uint32_t id = table[kt * kKvTile >> pool.shift]; id < uint32_t(pool.pages) && kt * kKvTile < most)
+        for (kt = masked0; kt < end; kt += TG)
+            if (const uint32_t id = page_of(kt); id < uint32_t(pool.pages))
 #pragma unroll
                 for (int q = 0; q < QT; ++q)
                     t[q].not_finite(pool.pool + pool.tile_at(id, job.head, 1, kt * kKvTile, TB), kt * kKvTile, s.ctx);
-
-    // the halves meet: the second one's out in LDS, [row group][QT][NU][lane]
-    f4_t *const so = reinterpret_cast<f4_t *>(&lds[0][0][0][0]) + rg * QT * NU * 64 + lane;
-    __syncthreads();
-    float l[QT];
+    // the results of the waves with the same rows meet in LDS
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-        l[q] = t[q].finish();
-        if (kg == 1 && lane < kRows) {
-            sml[0][rg][q][lane] = t[q].m;
-            sml[1][rg][q][lane] = l[q];
+        const float l = t[q].finish();
+        if (lane < kRows) {
+            sm[tg][rg][q][lane] = t[q].m;
+            sl[tg][rg][q][lane] = l;
         }
-        if (kg == 1) {
 #pragma unroll
-            for (int u = 0; u < NU; ++u) so[(q * NU + u) * 64] = t[q].o[u];
-        }
+        for (int u = 0; u < NU; ++u) so[tg][rg][q][u][lane] = t[q].o[u];
     }
     __syncthreads();
-    if (!busy || kg == 1) return;
+    const int lr = lane & 15;
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-        const int mine = row0 + q * kRows + (lane & 15);
-        const float m1 = sml[0][rg][q][lane & 15], l1 = sml[1][rg][q][lane & 15], m = fmaxf(t[q].m, m1);
-        // a half that saw no token adds nothing, whatever its zeros would be multiplied by
-        const bool h0 = l[q] != 0.f, h1 = l1 != 0.f;
-        const float f0 = t[q].m == m ? 1.f : __builtin_amdgcn_exp2f(t[q].m - m);
-        const float f1 = m1 == m ? 1.f : __builtin_amdgcn_exp2f(m1 - m);
-        const float sum = (h0 ? l[q] * f0 : 0.f) + (h1 ? l1 * f1 : 0.f);
-        if (mine < rows) {
+        const int row = row0 + q * kRows + lr;
+        float m = -INFINITY, l = 0.f, f[TG];
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                f4_t o = {0.f, 0.f, 0.f, 0.f};
-                if (h0) o += t[q].o[u] * f0;
-                if (h1) o += so[(q * NU + u) * 64] * f1;
-                put_row<HD>(a, job, splits, mine, u, lane, o, m, sum);
-            }
+        for (int k = 0; k < TG; ++k) m = fmaxf(m, sm[k][rg][q][lr]);
+#pragma unroll
+        for (int k = 0; k < TG; ++k) {
+            // a wave that saw no token adds nothing, whatever its zeros would be multiplied by
+            const float lk = sl[k][rg][q][lr], mk = sm[k][rg][q][lr];
+            f[k] = lk == 0.f ? 0.f : mk == m ? 1.f : __builtin_amdgcn_exp2f(mk - m);
+            l += lk == 0.f ? 0.f : f[k] * lk;
+        }
+        if (row >= rows) continue;
+        for (int u = tg; u < NU; u += TG) {
+            f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < TG; ++k)
+                if (sl[k][rg][q][lr] != 0.f) o += so[k][rg][q][u][lane] * f[k];
+            put_row<HD>(a, job, splits, row, u, lane, o, m, l);
         }
     }
 }
@@ -735,24 +589,22 @@ __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows
         if (HD >= 64 || lane < HD) out[64 * n + lane] = l == 0.f ? 0.f : o[n] / l;
 }
 
-// How a call is cut: sequences of up to kRows rows to a K/V head (group * rows) to k_attn_rows, the
-// others to k_attn_chunk, and the tokens of both into `splits` shares: enough workgroups to fill the
-// GPU, and none with fewer than 256 tokens.
+// How a call is cut: sequences of up to kRows rows to a K/V head (group * rows) are one launch's, the
+// others another's, and the tokens of both go into `splits` shares: as many as fill the GPU's compute
+// units (few rows: twice, so that sequences of different lengths even out), none under 256 tokens.
 struct Plan {
-    int splits, chunk_tiles;
-    bool rows, chunk;
+    int splits, tiles;  // shares; row tiles of the second launch
+    bool few, many;
 };
+constexpr int kManyRows = 64;  // of a workgroup of the second launch: RG 2, and QT 2 (hd 256: RG 4, QT 1)
 Plan plan(const KvPool &p, int hd, int heads, int max_new, int max_ctx, bool uniform) {
     Plan c;
-    const int group = heads / p.heads;
-    const long long most = (long long)max_new * group, wg = hd <= 128 ? 128 : 64;
-    c.chunk = most > kRows;
-    c.rows = !c.chunk || !uniform;
-    c.chunk_tiles = int((most + wg - 1) / wg);
-    const long long jobs = (long long)p.seqs * p.heads * (c.chunk ? c.chunk_tiles : 1);
-    // workgroups that the 256 CUs hold at once, and of k_attn_rows twice as many, so that sequences of
-    // different lengths even out
-    const int fit = c.chunk ? (hd <= 64 ? 2 : 1) : 2 * (hd <= 64 ? 3 : hd <= 128 ? 2 : 1);
+    const long long most = (long long)max_new * (heads / p.heads);
+    c.many = most > kRows;
+    c.few = !c.many || !uniform;
+    c.tiles = int((most + kManyRows - 1) / kManyRows);
+    const long long jobs = (long long)p.seqs * p.heads * (c.many ? c.tiles : 1);
+    const int fit = c.many ? 2 : 2 * (hd <= 64 ? 3 : hd <= 128 ? 2 : 1);
     long long s = 256 * fit / jobs;
     s = s < max_ctx / 256 ? s : max_ctx / 256;
     c.splits = s < 1 ? 1 : int(s);
@@ -772,15 +624,18 @@ template <int HD, bool Q8>
 hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx, hipStream_t st) {
     const int group = a.heads / p.heads;
     const Plan c = plan(p, HD, a.heads, r.max_new, max_ctx, !r.row_off);
-    const long long pairs = (long long)p.seqs * p.heads * c.splits, chunks = pairs * c.chunk_tiles;
+    const long long pairs = (long long)p.seqs * p.heads * c.splits, many = pairs * c.tiles;
     const long long joins = ((long long)p.seqs * r.max_new * a.heads + kWaves - 1) / kWaves;
-    if (pairs > 0x7fffffffll || chunks > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
-    if (c.chunk)
-        hipLaunchKernelGGL((k_attn_chunk<HD, Q8>), dim3(unsigned(chunks)), dim3(512), 0, st, p, a, r, group,
-                           c.chunk_tiles, c.splits, c.rows ? kRows : 0);
-    if (c.rows)
-        hipLaunchKernelGGL((k_attn_rows<HD, Q8>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p, a, r, group,
-                           c.splits);
+    if (pairs > 0x7fffffffll || many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
+    constexpr int kAll = 0x7fffffff;
+    if (c.many) {
+        constexpr int QT = HD <= 128 ? 2 : 1, RG = kManyRows / (QT * kRows), TG = HD <= 128 ? 2 : 1;
+        hipLaunchKernelGGL((k_attn<HD, Q8, QT, RG, TG>), dim3(unsigned(many)), dim3(64 * RG * TG), 0, st, p, a, r, group,
+                           c.tiles, c.splits, c.few ? kRows : 0, kAll);
+    }
+    if (c.few)
+        hipLaunchKernelGGL((k_attn<HD, Q8, 1, 1, kWaves>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p, a, r,
+                           group, 1, c.splits, 0, kRows);
     if (c.splits > 1)
         hipLaunchKernelGGL((k_attn_join<HD>), dim3(unsigned(joins)), dim3(64 * kWaves), 0, st, p, a, r, c.splits);
     return hipGetLastError();
