@@ -20,11 +20,17 @@
 namespace mlg {
 namespace {
 
+#ifndef MLG_FEW
+#define MLG_FEW 2048
+#define MLG_MANY 2048
+#endif
 constexpr int kRows = 16;        // rows of a query tile (columns of the matrix products)
 constexpr int kWaves = 4;        // waves of a workgroup
 // p = 2^(s - m): m is the running maximum of the scores (log2 units) less kPShift, and follows a larger
 // one only when it is kPSlack or more behind, which after the first tiles is rare: p stays below 2^15.
 constexpr float kPShift = 7.f, kPSlack = 8.f;
+
+constexpr int kLeastTiles = 8;  // of a split: a short sequence does not use all of a call's splits
 
 // Partial result of a split: [m, l, -, -, out of HD dims] of one row, f32, as a Tile holds them.
 constexpr int kPartHead = 4;
@@ -85,42 +91,25 @@ __device__ __forceinline__ uint32_t rows_umax(uint32_t v) {
 // One lane's part of a K or V tile, as it lies in the cache.
 template <int HD, bool Q8>
 struct RawTile {
-    static constexpr int NC = HD / 32, NP = Q8 ? NC : 2 * NC, ND = Q8 ? NC : 1;
-    uint4 a[NP];
-    uint4 d[ND];  // q8_0: the scales of the lane's tokens 8 g .. 8 g + 7, per block of 32 dims
+    static constexpr int NC = HD / 32, NU = HD / 16, NP = Q8 ? NC : NU, ND = Q8 ? NC : 1;
+    u4_t a[NP];
+    u4_t d[ND];  // q8_0: the scales of the lane's tokens 8 g .. 8 g + 7, per block of 32 dims
     __device__ __forceinline__ void load(const uint8_t *tile, int lane) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const uint4 *>(tile + (i * 64 + lane) * 16);
+        for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const u4_t *>(tile + (i * 64 + lane) * 16);
         if constexpr (Q8) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
-                d[c] = *reinterpret_cast<const uint4 *>(tile + kv_scale_byte(HD, 8 * (lane >> 4), c));
+                d[c] = *reinterpret_cast<const u4_t *>(tile + kv_scale_byte(HD, 8 * (lane >> 4), c));
         }
     }
-};
-
-// The same as matrix operands: K's product b of dims 32 c .. at 2 c + b, V's dims 16 u .. at u.
-template <int HD, bool Q8>
-struct Frags {
-    static constexpr int NC = HD / 32, NU = HD / 16;
-    h8_t a[NU];
-    uint4 d[Q8 ? NC : 1];
-    __device__ __forceinline__ void from(const RawTile<HD, Q8> &r) {
-        if constexpr (Q8) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                a[2 * c] = i8_to_h8(r.a[c].x, r.a[c].y);
-                a[2 * c + 1] = i8_to_h8(r.a[c].z, r.a[c].w);
-                d[c] = r.d[c];
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < NU; ++u) a[u] = as_h8(r.a[u]);
-        }
+    // As a matrix operand: K's product b of dims 32 c .. at 2 c + b, V's dims 16 u .. at u.
+    __device__ __forceinline__ h8_t frag(int i) const {
+        if constexpr (Q8) return i8_to_h8(a[i >> 1][2 * (i & 1)], a[i >> 1][2 * (i & 1) + 1]);
+        else return __builtin_bit_cast(h8_t, a[i]);
     }
     __device__ __forceinline__ float scale(int c, int n) const {
-        const uint32_t w[4] = {d[c].x, d[c].y, d[c].z, d[c].w};
-        return float(__builtin_bit_cast(h2_t, w[n >> 1])[n & 1]);
+        return float(__builtin_bit_cast(h2_t, uint32_t(d[c][n >> 1]))[n & 1]);
     }
     // V's tokens past the first `keep` of the lane's eight as zeros (of q8_0, their scales): they are
     // whatever the page held before. f16: what is left of inf and NaN as zeros too, which 0 would turn
@@ -130,21 +119,44 @@ struct Frags {
         constexpr int N = Q8 ? NC : NU;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint4 v = Q8 ? d[Q8 ? i : 0] : __builtin_bit_cast(uint4, a[i]);
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                w[n] = keep > 2 * n + 1 ? w[n] : keep > 2 * n ? w[n] & 0xffffu : 0u;
-                if constexpr (!Q8) {
-                    const bool lo = (w[n] & 0x7c00u) == 0x7c00u, hi = (w[n] & 0x7c000000u) == 0x7c000000u;
+                uint32_t w = Q8 ? d[Q8 ? i : 0][n] : a[Q8 ? 0 : i][n];
+                w = keep > 2 * n + 1 ? w : keep > 2 * n ? w & 0xffffu : 0u;
+                if constexpr (Q8) {
+                    d[i][n] = w;
+                } else {
+                    const bool lo = (w & 0x7c00u) == 0x7c00u, hi = (w & 0x7c000000u) == 0x7c000000u;
                     odd |= lo || hi;
-                    w[n] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                    a[i][n] = w & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
                 }
             }
-            if constexpr (Q8) d[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            else a[i] = as_h8(make_uint4(w[0], w[1], w[2], w[3]));
         }
         return odd;
+    }
+    // q8_0, V: the exponent of the largest scale of the tile's tokens (INT_MIN: all zeros), inf and NaN
+    // left out; subnormals count as the smallest normal one.
+    __device__ __forceinline__ int top_exponent() const {
+        // f16 bit patterns of scales, which are not negative, are ordered; two at once
+        typedef uint16_t u2_t __attribute__((ext_vector_type(2)));
+        u2_t t2 = {0, 0};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) t2 = __builtin_elementwise_max(t2, __builtin_bit_cast(u2_t, uint32_t(d[c][n])));
+        uint32_t top = rows_umax(max(uint32_t(t2[0]), uint32_t(t2[1])));
+        if (__any(top >= 0x7c00u)) {
+            top = 0u;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const uint32_t b = d[c][n >> 1] >> (16 * (n & 1)) & 0xffffu;
+                    top = max(top, b >= 0x7c00u ? 0u : b);
+                }
+            top = rows_umax(top);
+        }
+        return top ? max(int(top >> 10), 1) - 15 : int(0x80000000);
     }
 };
 
@@ -180,8 +192,7 @@ struct Tile {
     int vis;     // tokens that this lane's row sees
     float m;     // the running maximum (log2 units) less kPShift, as rounded: p = 2^(s - m)
     f4_t l;      // f16: sum of p over all tokens so far, in each element; q8_0: l[0] over the lane's
-    f4_t o[NU];
-    int e;       // q8_0: out is held times 2^-e (e: the largest exponent of V's scales so far)
+    f4_t o[NU];  // q8_0: times 2^-e of its Rows
 
     // q: the row's HD values (null: a row past the last, as zeros)
     __device__ __forceinline__ void load_q(const float *q, float scale, int lane) {
@@ -216,28 +227,8 @@ struct Tile {
             }
         m = -INFINITY;
         l = f4_t{0.f, 0.f, 0.f, 0.f};
-        e = -100;
 #pragma unroll
         for (int u = 0; u < NU; ++u) o[u] = f4_t{0.f, 0.f, 0.f, 0.f};
-    }
-
-    // The lane's 8 products (tokens 8 g .. 8 g + 7 of the tile, its row), not yet times qf.
-    __device__ __forceinline__ void scores(const Frags<HD, Q8> &k, float (&s)[8]) const {
-        f4_t acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                if constexpr (Q8) {
-                    f4_t t = mfma(k.a[2 * c + b], qh[c], mfma(k.a[2 * c + b], ql[c], f4_t{0.f, 0.f, 0.f, 0.f}));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[b][i] = fmaf(t[i], k.scale(c, 4 * b + i), acc[b][i]);
-                } else {
-                    acc[b] = mfma(k.a[2 * c + b], qh[c], mfma(k.a[2 * c + b], ql[c], acc[b]));
-                }
-            }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) s[n] = acc[n >> 2][n & 3];
     }
 
     // The largest score of the lane's row in a tile, as m holds it.
@@ -263,75 +254,6 @@ struct Tile {
         if constexpr (Q8) l[0] += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     }
 
-    // q8_0: out follows a larger scale of V than any before, so that p times a scale stays within
-    // f16's range (below 2^16) and keeps its bits whatever the scales' size.
-    __device__ __forceinline__ void fit(const Frags<HD, Q8> &v) {
-        // f16 bit patterns of scales that are not negative are ordered; two at once
-        typedef uint16_t u2_t __attribute__((ext_vector_type(2)));
-        u2_t t2 = {0, 0};
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const uint32_t w[4] = {v.d[c].x, v.d[c].y, v.d[c].z, v.d[c].w};
-#pragma unroll
-            for (int n = 0; n < 4; ++n) t2 = __builtin_elementwise_max(t2, __builtin_bit_cast(u2_t, w[n]));
-        }
-        uint32_t top = rows_umax(max(uint32_t(t2[0]), uint32_t(t2[1])));
-        if (__any(top >= 0x7c00u)) {  // inf, NaN (no scale is negative): the other tokens' rows go on
-            top = 0u;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const uint32_t w[4] = {v.d[c].x, v.d[c].y, v.d[c].z, v.d[c].w};
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const uint32_t b = w[n >> 1] >> (16 * (n & 1)) & 0xffffu;
-                    top = max(top, b >= 0x7c00u ? 0u : b);
-                }
-            }
-            top = rows_umax(top);
-        }
-        // the exponent of an f16; subnormals count as the smallest normal one
-        const int x = top ? max(int(top >> 10), 1) - 15 : e;
-        if (__any(x > e)) {
-            const int en = max(e, x);
-            const float f = ldexpf(1.f, max(e - en, -126));
-#pragma unroll
-            for (int u = 0; u < NU; ++u) o[u] *= f;
-            e = en;
-        }
-    }
-
-    // out += p V. MASKED: tokens whose p is 0 here may hold anything, inf and NaN among it.
-    template <bool MASKED>
-    __device__ __forceinline__ void values(const Frags<HD, Q8> &v, const float (&p)[8]) {
-        h8_t ph, pl;
-        if constexpr (Q8) {
-            fit(v);
-            const float down = ldexpf(1.f, -e);
-            float pe[8];
-#pragma unroll
-            for (int n = 0; n < 8; ++n) pe[n] = p[n] * down;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float pd[8];
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    pd[n] = fmaf(pe[n], v.scale(c, n), 0.f);
-                    if (MASKED && p[n] == 0.f) pd[n] = 0.f;
-                }
-                split8(pd, ph, pl);
-#pragma unroll
-                for (int u = 2 * c; u < 2 * c + 2; ++u) o[u] = mfma(v.a[u], ph, mfma(v.a[u], pl, o[u]));
-            }
-        } else {
-            split8(p, ph, pl);
-            const _Float16 w = _Float16(1.f);
-            const h8_t one = {w, w, w, w, w, w, w, w};
-            l = mfma(one, ph, mfma(one, pl, l));
-#pragma unroll
-            for (int u = 0; u < NU; ++u) o[u] = mfma(v.a[u], ph, mfma(v.a[u], pl, o[u]));
-        }
-    }
-
     // f16, after the last tile: the inf and NaN that cut() took out of one tile's V, to the rows that
     // see their tokens (tile: V of tokens tok0 .. in the cache). Not met by ordinary caches.
     __device__ __forceinline__ void not_finite(const uint8_t *tile, int tok0, int ctx) {
@@ -354,17 +276,129 @@ struct Tile {
 #pragma unroll
         for (int n = 0; n < 8; ++n) s[n] = at + n < vis ? s[n] : -INFINITY;
     }
+};
 
-    // After the last tile: l as one sum of the row, out as it is.
-    __device__ __forceinline__ float finish() {
+// A wave's QT tiles of rows: the matrix products, a K or V operand at a time for all of them.
+template <int HD, bool Q8, int QT>
+struct Rows {
+    static constexpr int NC = HD / 32, NU = HD / 16;
+    Tile<HD, Q8> t[QT];
+    int e = -100;  // q8_0: the largest exponent of V's scales so far
+
+    // The lane's 8 products (tokens 8 g .. 8 g + 7 of the tile) for its row of each tile, not yet times qf.
+    __device__ __forceinline__ void scores(const RawTile<HD, Q8> &k, float (&s)[QT][8]) const {
+        f4_t acc[QT][2];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) acc[q][0] = acc[q][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const h8_t kf = k.frag(2 * c + b);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                    if constexpr (Q8) {
+                        const f4_t x = mfma(kf, t[q].qh[c], mfma(kf, t[q].ql[c], f4_t{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[q][b][i] = fmaf(x[i], k.scale(c, 4 * b + i), acc[q][b][i]);
+                    } else {
+                        acc[q][b] = mfma(kf, t[q].qh[c], mfma(kf, t[q].ql[c], acc[q][b]));
+                    }
+                }
+            }
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) s[q][n] = acc[q][n >> 2][n & 3];
+    }
+
+    // m follows the tile's scores where a row's p would grow too large.
+    __device__ __forceinline__ void follow(const float (&s)[QT][8]) {
+        float top[QT];
+        bool behind = false;
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            top[q] = t[q].top(s[q]);
+            behind |= t[q].behind(top[q]);
+        }
+        if (__any(behind)) {  // wave-uniform
+#pragma unroll
+            for (int q = 0; q < QT; ++q) t[q].follow(top[q]);
+        }
+    }
+
+    // q8_0: out follows a larger scale of V than any before, so that p times a scale stays within
+    // f16's range (below 2^16) and keeps its bits whatever the scales' size.
+    __device__ __forceinline__ void fit(const RawTile<HD, Q8> &v) {
+        const int x = v.top_exponent();
+        if (__any(x > e)) {
+            const float f = ldexpf(1.f, max(e - x, -126));
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+#pragma unroll
+                for (int u = 0; u < NU; ++u) t[q].o[u] *= f;
+            e = x;
+        }
+    }
+
+    // s becomes p, out += p V. MASKED: tokens whose p is 0 here may hold anything, inf and NaN among it.
+    template <bool MASKED>
+    __device__ __forceinline__ void values(const RawTile<HD, Q8> &v, float (&s)[QT][8]) {
+        if constexpr (Q8) {
+            fit(v);
+            const float down = ldexpf(1.f, -e);
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                t[q].probs(s[q]);
+#pragma unroll
+                for (int n = 0; n < 8; ++n) s[q][n] *= down;
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const h8_t vf[2] = {v.frag(2 * c), v.frag(2 * c + 1)};
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                    float pd[8];
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        pd[n] = fmaf(s[q][n], v.scale(c, n), 0.f);
+                        if (MASKED && s[q][n] == 0.f) pd[n] = 0.f;
+                    }
+                    h8_t ph, pl;
+                    split8(pd, ph, pl);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        t[q].o[2 * c + u] = mfma(vf[u], ph, mfma(vf[u], pl, t[q].o[2 * c + u]));
+                }
+            }
+        } else {
+            const _Float16 w = _Float16(1.f);
+            const h8_t one = {w, w, w, w, w, w, w, w};
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                t[q].probs(s[q]);
+                h8_t ph, pl;
+                split8(s[q], ph, pl);
+                t[q].l = mfma(one, ph, mfma(one, pl, t[q].l));
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    const h8_t vf = v.frag(u);
+                    t[q].o[u] = mfma(vf, ph, mfma(vf, pl, t[q].o[u]));
+                }
+            }
+        }
+    }
+
+    // After the last tile: a row's l as one sum, its out as it is.
+    __device__ __forceinline__ float finish(int q) {
         if constexpr (Q8) {
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) o[u][n] = ldexpf(o[u][n], e);
-            return rows_sum(l[0]);
+                for (int n = 0; n < 4; ++n) t[q].o[u][n] = ldexpf(t[q].o[u][n], e);
+            return rows_sum(t[q].l[0]);
         }
-        return l[0];
+        return t[q].l[0];
     }
 };
 
@@ -391,7 +425,7 @@ __device__ __forceinline__ void put_row(const KvAttn &a, const Work &w, int spli
     } else {
         float *part = a.scratch + ((w.qrow(row) * size_t(a.heads) + size_t(w.qhead(row))) * size_t(splits) +
                                    size_t(w.split)) * size_t(HD + kPartHead);
-        *reinterpret_cast<f4_t *>(part + kPartHead + dim) = o;
+        if (l != 0.f) *reinterpret_cast<f4_t *>(part + kPartHead + dim) = o;
         if (u == 0 && lane < kRows) {
             part[0] = m;
             part[1] = l;
@@ -410,7 +444,7 @@ template <int HD, bool Q8, int QT, int RG, int TG>
 struct Shape {
     static constexpr int kRowsWg = RG * QT * kRows, kThreads = 64 * RG * TG;
     // waves of a SIMD: what the registers of a wave leave room for
-    static constexpr int kWavesSimd = QT == 1 ? (HD <= 64 ? 3 : HD <= 128 ? 2 : 1) : (HD <= 64 ? 3 : 2);
+    static constexpr int kWavesSimd = QT == 1 ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 1) : (HD <= 64 ? 3 : 2);
 };
 
 template <int HD, bool Q8, int QT, int RG, int TG>
@@ -441,7 +475,8 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
     const bool busy = row0 < rows;
     // what the wave's first and last row see
     const int least = job.sees(a, min(row0, rows - 1)), most = busy ? job.sees(a, min(row0 + QT * kRows, rows) - 1) : 0;
-    Tile<HD, Q8> t[QT];
+    Rows<HD, Q8, QT> wave;
+    Tile<HD, Q8>(&t)[QT] = wave.t;
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
         const int mine = row0 + j * kRows + (lane & 15), row = min(mine, rows - 1);
@@ -450,7 +485,7 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
     }
     // the split's tiles: the same for all of a workgroup's rows
     const int all = (job.sees(a, min(first + S::kRowsWg, rows) - 1) + kKvTile - 1) / kKvTile;
-    const int per = (all + splits - 1) / splits;
+    const int per = max((all + splits - 1) / splits, kLeastTiles);
     const int end = min((most + kKvTile - 1) / kKvTile, (job.split + 1) * per);
     const uint32_t *table = pool.table + size_t(job.i) * size_t(pool.table_len);
     RawTile<HD, Q8> kr, vr;
@@ -471,39 +506,19 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
         const int tok0 = kt * kKvTile;
         const bool there = page < uint32_t(pool.pages);
         float p[QT][8];
-        Frags<HD, Q8> f;
-        if (there) {
-            f.from(kr);
-#pragma unroll
-            for (int q = 0; q < QT; ++q) t[q].scores(f, p[q]);
-        } else if (r.bad && lane == 0) {  // its tokens are not there
-            *r.bad = 1u;
-        }
+        if (there) wave.scores(kr, p);
+        else if (r.bad && lane == 0) *r.bad = 1u;  // its tokens are not there
         load(kr, 0, next, kt + TG);
         if (there) {
-            float top[QT];
-            bool behind = false;
+            if constexpr (kMasked) {
 #pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                if constexpr (kMasked) t[q].hide(p[q], tok0);
-                top[q] = t[q].top(p[q]);
-                behind |= t[q].behind(top[q]);
+                for (int q = 0; q < QT; ++q) t[q].hide(p[q], tok0);
+                odd |= vr.cut(s.ctx - tok0 - 8 * (lane >> 4));
             }
-            if (__any(behind)) {  // wave-uniform
-#pragma unroll
-                for (int q = 0; q < QT; ++q) t[q].follow(top[q]);
-            }
-            f.from(vr);
+            wave.follow(p);
+            wave.template values<kMasked>(vr, p);
         }
         load(vr, 1, next, kt + TG);
-        if (there) {
-            if constexpr (kMasked) odd |= f.cut(s.ctx - tok0 - 8 * (lane >> 4));
-#pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                t[q].probs(p[q]);
-                t[q].template values<kMasked>(f, p[q]);
-            }
-        }
         page = next;
         next = page_of(kt + 2 * TG);
     };
@@ -520,7 +535,7 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
     // the results of the waves with the same rows meet in LDS
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-        const float l = t[q].finish();
+        const float l = wave.finish(q);
         if (lane < kRows) {
             sm[tg][rg][q][lane] = t[q].m;
             sl[tg][rg][q][lane] = l;
@@ -554,39 +569,68 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
     }
 }
 
-// The splits of a row joined in their order: a wave per (row, head).
+// The splits of a row joined in their order. A wave per (row, head): lane k weighs split k, all of their
+// m and l read at once; then the outs, 16 bytes a lane, as many splits at a time as a wave has lanes for.
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows r, int splits) {
+    constexpr int LANES = HD / 4, AT = 64 / LANES, PART = HD + kPartHead;  // lanes of an out; outs at a time
     const int lane = threadIdx.x & 63;
-    const size_t job = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-    const size_t per = size_t(r.max_new) * size_t(a.heads);
-    const int i = int(job / per);
-    if (i >= pool.seqs) return;
-    const KvSeq s = kv_seq(pool, r, i);
-    const int row = int(job % per / size_t(a.heads)), head = int(job % size_t(a.heads));
-    if (row >= s.n) return;
-    const size_t qrow = size_t(s.r0 + row);
-    const float *part = a.scratch + (qrow * size_t(a.heads) + size_t(head)) * size_t(splits) * size_t(HD + kPartHead);
-    float m = -INFINITY, l = 0.f;
-    for (int k = 0; k < splits; ++k) m = fmaxf(m, part[size_t(k) * (HD + kPartHead)]);
-    constexpr int ND = (HD + 63) / 64;
-    float o[ND];
-#pragma unroll
-    for (int n = 0; n < ND; ++n) o[n] = 0.f;
-    for (int k = 0; k < splits; ++k) {
-        const float *pk = part + size_t(k) * (HD + kPartHead);
-        const float mk = pk[0], lk = pk[1];
-        if (lk == 0.f) continue;  // no token of this split seen
-        const float f = mk == m ? 1.f : __builtin_amdgcn_exp2f(mk - m);
-        l += f * lk;
-#pragma unroll
-        for (int n = 0; n < ND; ++n)
-            if (HD >= 64 || lane < HD) o[n] += f * pk[kPartHead + 64 * n + lane];
+    const size_t job = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6), qrow = job / size_t(a.heads);
+    const int head = int(job % size_t(a.heads));
+    if (qrow >= size_t(r.rows)) return;
+    // the sequence that has the row; a row that is none's, or past max_new of its own, is left alone
+    bool mine = false;
+    for (int i0 = 0; i0 < pool.seqs && !mine; i0 += 64) {  // wave-uniform
+        const int i = i0 + lane;
+        bool in = false;
+        if (i < pool.seqs) {
+            const KvSeq s = kv_seq(pool, r, i);
+            in = qrow >= size_t(s.r0) && qrow < size_t(s.r0) + size_t(s.n);
+        }
+        mine = __any(in);
     }
-    float *out = a.out + qrow * a.ldo + size_t(head) * HD;
+    if (!mine) return;
+    const float *part = a.scratch + (qrow * size_t(a.heads) + size_t(head)) * size_t(splits) * size_t(PART);
+    float m = -INFINITY, l = 0.f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < splits; k0 += 64) {
+        const int n = min(64, splits - k0);
+        const float *pk = part + size_t(k0) * PART;
+        float mk = -INFINITY, lk = 0.f;
+        if (lane < n) {
+            mk = pk[size_t(lane) * PART];
+            lk = pk[size_t(lane) * PART + 1];
+        }
+        const float mn = fmaxf(m, wave_max(mk)), down = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        // a split that saw no token adds nothing (and has no out)
+        const float f = lk == 0.f ? 0.f : mk == mn ? 1.f : __builtin_amdgcn_exp2f(mk - mn);
+        l = (l == 0.f ? 0.f : l * down) + wave_sum(lk == 0.f ? 0.f : f * lk);
+        o *= down;
+        m = mn;
+        const int last = 64 - __builtin_clzll(__ballot(lk != 0.f) | 1ull);  // splits that have an out: below
+        for (int k = 0; k < last; k += 4 * AT) {
+            f4_t x[4];
+            float fk[4];
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
-        if (HD >= 64 || lane < HD) out[64 * n + lane] = l == 0.f ? 0.f : o[n] / l;
+            for (int j = 0; j < 4; ++j) {
+                const int z = k + j * AT + lane / LANES;
+                fk[j] = __shfl(f, z & 63);
+                const float lz = __shfl(lk, z & 63);  // all lanes
+                x[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+                if (z < last && lz != 0.f) x[j] = *reinterpret_cast<const f4_t *>(pk + size_t(z) * PART + kPartHead + 4 * (lane % LANES));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o += x[j] * fk[j];
+        }
+    }
+#pragma unroll
+    for (int d = LANES; d < 64; d *= 2)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) o[n] += __shfl_xor(o[n], d);
+    if (lane < LANES) {
+        const f4_t y = l == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : o / l;
+        *reinterpret_cast<f4_t *>(a.out + qrow * a.ldo + size_t(head) * HD + 4 * lane) = y;
+    }
 }
 
 // How a call is cut: sequences of up to kRows rows to a K/V head (group * rows) are one launch's, the
@@ -596,17 +640,19 @@ struct Plan {
     int splits, tiles;  // shares; row tiles of the second launch
     bool few, many;
 };
+constexpr int kFewJobs = MLG_FEW, kManyJobs = MLG_MANY;  // workgroups of a launch, about
 constexpr int kManyRows = 64;  // of a workgroup of the second launch: RG 2, and QT 2 (hd 256: RG 4, QT 1)
-Plan plan(const KvPool &p, int hd, int heads, int max_new, int max_ctx, bool uniform) {
+Plan plan(const KvPool &p, int heads, int rows, int max_new, int max_ctx, bool uniform) {
     Plan c;
     const long long most = (long long)max_new * (heads / p.heads);
     c.many = most > kRows;
     c.few = !c.many || !uniform;
     c.tiles = int((most + kManyRows - 1) / kManyRows);
-    const long long jobs = (long long)p.seqs * p.heads * (c.many ? c.tiles : 1);
-    const int fit = c.many ? 2 : 2 * (hd <= 64 ? 3 : hd <= 128 ? 2 : 1);
-    long long s = 256 * fit / jobs;
-    s = s < max_ctx / 256 ? s : max_ctx / 256;
+    // workgroups of the launch that has the most of the work: one for every 64 rows, at least one a sequence
+    const long long of_rows = ((long long)rows * (heads / p.heads) + kManyRows - 1) / kManyRows;
+    const long long jobs = (long long)p.heads * (c.many ? of_rows : p.seqs);
+    long long s = (c.many ? kManyJobs : kFewJobs) / jobs;
+    s = s < max_ctx / (c.many ? 512 : 256) ? s : max_ctx / (c.many ? 512 : 256);
     c.splits = s < 1 ? 1 : int(s);
     return c;
 }
@@ -615,7 +661,7 @@ Plan plan(const KvPool &p, int hd, int heads, int max_new, int max_ctx, bool uni
 
 size_t attn_paged_scratch(const KvPool &p, int hd, int heads, int rows, int max_new, int max_ctx) {
     if (p.seqs <= 0 || rows <= 0) return 0;
-    const int s = plan(p, hd, heads, max_new, max_ctx, false).splits;
+    const int s = plan(p, heads, rows, max_new, max_ctx, false).splits;
     return s == 1 ? 0 : size_t(rows) * size_t(heads) * size_t(s) * size_t(hd + kPartHead) * sizeof(float);
 }
 
@@ -623,9 +669,9 @@ namespace {
 template <int HD, bool Q8>
 hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx, hipStream_t st) {
     const int group = a.heads / p.heads;
-    const Plan c = plan(p, HD, a.heads, r.max_new, max_ctx, !r.row_off);
+    const Plan c = plan(p, a.heads, r.rows, r.max_new, max_ctx, !r.row_off);
     const long long pairs = (long long)p.seqs * p.heads * c.splits, many = pairs * c.tiles;
-    const long long joins = ((long long)p.seqs * r.max_new * a.heads + kWaves - 1) / kWaves;
+    const long long joins = ((long long)r.rows * a.heads + kWaves - 1) / kWaves;
     if (pairs > 0x7fffffffll || many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
     constexpr int kAll = 0x7fffffff;
     if (c.many) {
