@@ -759,7 +759,7 @@ size_t mlg_attn_paged_scratch(const mlg_kv_cache *c, int heads, int rows, int ma
     if (!c || mlg_kv_page_bytes(c->type, c->heads, c->head_size, c->page) < 0 || heads < 1 || heads % c->heads ||
         rows < 1 || max_new < 1 || c->seqs < 1 || c->table_len < 1)
         return 0;
-    return mlg::attn_paged_scratch(kv_pool(c), c->head_size, heads, rows, max_new, kv_max_ctx(c, max_ctx));
+    return mlg::attn_paged_scratch(kv_pool(c), c->type == MLG_Q8_0, c->head_size, heads, rows, max_new, kv_max_ctx(c, max_ctx));
 }
 
 int mlg_attn_paged(const mlg_kv_cache *c, const float *q, int64_t ldq, int heads, float scale, int causal,

@@ -89,18 +89,29 @@ __device__ __forceinline__ uint32_t rows_umax(uint32_t v) {
 }
 
 // One lane's part of a K or V tile, as it lies in the cache.
-template <int HD, bool Q8>
+//
+// BLOCKS (q8_0, 16 / (HD / 32) rows at most): column col of the products is one block of 32 dims, col %
+// (HD / 32), of row col / (HD / 32) instead of a row. Its q is zero outside of its block and its p is
+// times its block's scales, so that a lane applies the scales of its own block alone, once, where every
+// row's lane applies all blocks' scales in turn otherwise.
+template <int HD, bool Q8, bool BLOCKS>
 struct RawTile {
-    static constexpr int NC = HD / 32, NU = HD / 16, NP = Q8 ? NC : NU, ND = Q8 ? NC : 1;
+    static constexpr int NC = HD / 32, NU = HD / 16, NP = Q8 ? NC : NU, ND = Q8 && !BLOCKS ? NC : 1;
     u4_t a[NP];
     u4_t d[ND];  // q8_0: the scales of the lane's tokens 8 g .. 8 g + 7, per block of 32 dims
+    // ONCE: no other workgroup reads the tile, so it is not kept in the caches (non-temporal loads).
+    template <bool ONCE>
     __device__ __forceinline__ void load(const uint8_t *tile, int lane) {
+        auto at = [](const uint8_t *p) __attribute__((always_inline)) {
+            const u4_t *q = reinterpret_cast<const u4_t *>(p);
+            return ONCE ? __builtin_nontemporal_load(q) : *q;
+        };
 #pragma unroll
-        for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const u4_t *>(tile + (i * 64 + lane) * 16);
+        for (int i = 0; i < NP; ++i) a[i] = at(tile + (i * 64 + lane) * 16);
         if constexpr (Q8) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-                d[c] = *reinterpret_cast<const u4_t *>(tile + kv_scale_byte(HD, 8 * (lane >> 4), c));
+            for (int c = 0; c < ND; ++c)
+                d[c] = at(tile + kv_scale_byte(HD, 8 * (lane >> 4), BLOCKS ? (lane & 15) % NC : c));
         }
     }
     // As a matrix operand: K's product b of dims 32 c .. at 2 c + b, V's dims 16 u .. at u.
@@ -116,7 +127,7 @@ struct RawTile {
     // into NaN for the rows that do not see its token; whether there was any (see not_finite).
     __device__ __forceinline__ bool cut(int keep) {
         bool odd = false;
-        constexpr int N = Q8 ? NC : NU;
+        constexpr int N = Q8 ? ND : NU;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
 #pragma unroll
@@ -134,21 +145,21 @@ struct RawTile {
         }
         return odd;
     }
-    // q8_0, V: the exponent of the largest scale of the tile's tokens (INT_MIN: all zeros), inf and NaN
-    // left out; subnormals count as the smallest normal one.
+    // q8_0, V: the exponent of the largest scale of the tile's tokens (INT_MIN: all zeros), of the lane's
+    // block where it has one, inf and NaN left out; subnormals count as the smallest normal one.
     __device__ __forceinline__ int top_exponent() const {
         // f16 bit patterns of scales, which are not negative, are ordered; two at once
         typedef uint16_t u2_t __attribute__((ext_vector_type(2)));
         u2_t t2 = {0, 0};
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < ND; ++c)
 #pragma unroll
             for (int n = 0; n < 4; ++n) t2 = __builtin_elementwise_max(t2, __builtin_bit_cast(u2_t, uint32_t(d[c][n])));
         uint32_t top = rows_umax(max(uint32_t(t2[0]), uint32_t(t2[1])));
         if (__any(top >= 0x7c00u)) {
             top = 0u;
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < ND; ++c)
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
                     const uint32_t b = d[c][n >> 1] >> (16 * (n & 1)) & 0xffffu;
@@ -183,8 +194,18 @@ __device__ __forceinline__ f4_t mfma(const h8_t &a, const h8_t &b, const f4_t &c
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// A tile of 16 rows, and the softmax and sums of what it has seen.
-template <int HD, bool Q8>
+// Sum (MAX: maximum) over the columns of a row: N = 1, 2, 4 or 8 neighbouring lanes.
+template <int N, bool MAX>
+__device__ __forceinline__ float over_columns(float v) {
+    auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+    if constexpr (N >= 2) v = op(v, dpp_mov<kDppXor1>(v));
+    if constexpr (N >= 4) v = op(v, dpp_mov<kDppXor2>(v));
+    if constexpr (N >= 8) v = op(v, dpp_mov<kDppHalfMirror>(v));
+    return v;
+}
+
+// A tile of 16 columns (rows, or blocks of rows), and the softmax and sums of what it has seen.
+template <int HD, bool Q8, bool BLOCKS>
 struct Tile {
     static constexpr int NC = HD / 32, NU = HD / 16;
     h8_t qh[NC], ql[NC];
@@ -192,7 +213,8 @@ struct Tile {
     int vis;     // tokens that this lane's row sees
     float m;     // the running maximum (log2 units) less kPShift, as rounded: p = 2^(s - m)
     f4_t l;      // f16: sum of p over all tokens so far, in each element; q8_0: l[0] over the lane's
-    f4_t o[NU];  // q8_0: times 2^-e of its Rows
+    f4_t o[NU];
+    int e = -100;  // q8_0: the largest exponent of V's scales so far; p, l and out are held times 2^-e
 
     // q: the row's HD values (null: a row past the last, as zeros)
     __device__ __forceinline__ void load_q(const float *q, float scale, int lane) {
@@ -208,6 +230,10 @@ struct Tile {
             x[c][4] = b.x, x[c][5] = b.y, x[c][6] = b.z, x[c][7] = b.w;
 #pragma unroll
             for (int n = 0; n < 8; ++n) amax = fmaxf(amax, fabsf(x[c][n]));
+            if (BLOCKS && c != (lane & 15) % NC) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) x[c][n] = 0.f;
+            }
         }
         amax = rows_max(amax);
         // the row's largest value to [2^14, 2^15); not for 0, inf (NaN is not seen by the maximum)
@@ -248,7 +274,7 @@ struct Tile {
     }
     // s becomes p.
     __device__ __forceinline__ void probs(float (&s)[8]) {
-        const float base = m == -INFINITY ? 0.f : m;  // nothing seen: every score is -inf
+        const float base = (m == -INFINITY ? 0.f : m) + (Q8 ? float(e) : 0.f);  // -inf: every score is -inf
 #pragma unroll
         for (int n = 0; n < 8; ++n) s[n] = __builtin_amdgcn_exp2f(fmaf(s[n], qf, -base));
         if constexpr (Q8) l[0] += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
@@ -279,14 +305,14 @@ struct Tile {
 };
 
 // A wave's QT tiles of rows: the matrix products, a K or V operand at a time for all of them.
-template <int HD, bool Q8, int QT>
+template <int HD, bool Q8, bool BLOCKS, int QT>
 struct Rows {
     static constexpr int NC = HD / 32, NU = HD / 16;
-    Tile<HD, Q8> t[QT];
-    int e = -100;  // q8_0: the largest exponent of V's scales so far
+    typedef RawTile<HD, Q8, BLOCKS> Raw;
+    Tile<HD, Q8, BLOCKS> t[QT];
 
     // The lane's 8 products (tokens 8 g .. 8 g + 7 of the tile) for its row of each tile, not yet times qf.
-    __device__ __forceinline__ void scores(const RawTile<HD, Q8> &k, float (&s)[QT][8]) const {
+    __device__ __forceinline__ void scores(const Raw &k, float (&s)[QT][8]) const {
         f4_t acc[QT][2];
 #pragma unroll
         for (int q = 0; q < QT; ++q) acc[q][0] = acc[q][1] = f4_t{0.f, 0.f, 0.f, 0.f};
@@ -297,7 +323,7 @@ struct Rows {
                 const h8_t kf = k.frag(2 * c + b);
 #pragma unroll
                 for (int q = 0; q < QT; ++q) {
-                    if constexpr (Q8) {
+                    if constexpr (Q8 && !BLOCKS) {
                         const f4_t x = mfma(kf, t[q].qh[c], mfma(kf, t[q].ql[c], f4_t{0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[q][b][i] = fmaf(x[i], k.scale(c, 4 * b + i), acc[q][b][i]);
@@ -309,7 +335,10 @@ struct Rows {
 #pragma unroll
         for (int q = 0; q < QT; ++q)
 #pragma unroll
-            for (int n = 0; n < 8; ++n) s[q][n] = acc[q][n >> 2][n & 3];
+            for (int n = 0; n < 8; ++n) {
+                s[q][n] = acc[q][n >> 2][n & 3];
+                if constexpr (BLOCKS) s[q][n] = over_columns<NC, false>(fmaf(s[q][n], k.scale(0, n), 0.f));
+            }
     }
 
     // m follows the tile's scores where a row's p would grow too large.
@@ -327,45 +356,47 @@ struct Rows {
         }
     }
 
-    // q8_0: out follows a larger scale of V than any before, so that p times a scale stays within
+    // q8_0: l and out follow a larger scale of V than any before, so that p times a scale stays within
     // f16's range (below 2^16) and keeps its bits whatever the scales' size.
-    __device__ __forceinline__ void fit(const RawTile<HD, Q8> &v) {
+    __device__ __forceinline__ void fit(const Raw &v) {
         const int x = v.top_exponent();
-        if (__any(x > e)) {
-            const float f = ldexpf(1.f, max(e - x, -126));
+        if (__any(x > t[0].e)) {
+            const int en = max(x, t[0].e);
+            const float f = ldexpf(1.f, max(t[0].e - en, -126));
 #pragma unroll
-            for (int q = 0; q < QT; ++q)
+            for (int q = 0; q < QT; ++q) {
+                t[q].l *= f;
 #pragma unroll
                 for (int u = 0; u < NU; ++u) t[q].o[u] *= f;
-            e = x;
+                t[q].e = en;
+            }
         }
     }
 
     // s becomes p, out += p V. MASKED: tokens whose p is 0 here may hold anything, inf and NaN among it.
     template <bool MASKED>
-    __device__ __forceinline__ void values(const RawTile<HD, Q8> &v, float (&s)[QT][8]) {
+    __device__ __forceinline__ void values(const Raw &v, float (&s)[QT][8]) {
         if constexpr (Q8) {
             fit(v);
-            const float down = ldexpf(1.f, -e);
 #pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                t[q].probs(s[q]);
+            for (int q = 0; q < QT; ++q) t[q].probs(s[q]);
+            auto scaled = [&](int q, int c, h8_t &ph, h8_t &pl) __attribute__((always_inline)) {
+                float pd[8];
 #pragma unroll
-                for (int n = 0; n < 8; ++n) s[q][n] *= down;
-            }
+                for (int n = 0; n < 8; ++n) {
+                    pd[n] = fmaf(s[q][n], v.scale(c, n), 0.f);
+                    if (MASKED && s[q][n] == 0.f) pd[n] = 0.f;
+                }
+                split8(pd, ph, pl);
+            };
+            h8_t ph, pl;
+            if constexpr (BLOCKS) scaled(0, 0, ph, pl);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const h8_t vf[2] = {v.frag(2 * c), v.frag(2 * c + 1)};
 #pragma unroll
                 for (int q = 0; q < QT; ++q) {
-                    float pd[8];
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        pd[n] = fmaf(s[q][n], v.scale(c, n), 0.f);
-                        if (MASKED && s[q][n] == 0.f) pd[n] = 0.f;
-                    }
-                    h8_t ph, pl;
-                    split8(pd, ph, pl);
+                    if constexpr (!BLOCKS) scaled(q, c, ph, pl);
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
                         t[q].o[2 * c + u] = mfma(vf[u], ph, mfma(vf[u], pl, t[q].o[2 * c + u]));
@@ -395,8 +426,8 @@ struct Rows {
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) t[q].o[u][n] = ldexpf(t[q].o[u][n], e);
-            return rows_sum(t[q].l[0]);
+                for (int n = 0; n < 4; ++n) t[q].o[u][n] = ldexpf(t[q].o[u][n], t[q].e);
+            return ldexpf(rows_sum(t[q].l[0]), t[q].e);
         }
         return t[q].l[0];
     }
@@ -418,6 +449,7 @@ struct Work {
 template <int HD>
 __device__ __forceinline__ void put_row(const KvAttn &a, const Work &w, int splits, int row, int u, int lane,
                                         const f4_t &o, float m, float l) {
+    // m and l of a row are written once, with its dims 0 .. 3
     const int dim = 16 * u + 4 * (lane >> 4);
     if (splits == 1) {
         const f4_t y = l == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : o / l;
@@ -426,7 +458,7 @@ __device__ __forceinline__ void put_row(const KvAttn &a, const Work &w, int spli
         float *part = a.scratch + ((w.qrow(row) * size_t(a.heads) + size_t(w.qhead(row))) * size_t(splits) +
                                    size_t(w.split)) * size_t(HD + kPartHead);
         if (l != 0.f) *reinterpret_cast<f4_t *>(part + kPartHead + dim) = o;
-        if (u == 0 && lane < kRows) {
+        if (dim == 0) {
             part[0] = m;
             part[1] = l;
         }
@@ -440,17 +472,19 @@ __device__ __forceinline__ void put_row(const KvAttn &a, const Work &w, int spli
 // LDS that eight waves shared measured slower: 298 to 376 us against the 4001-token chunk's figure
 // below, for its barriers and because a stage is worked on in less time than the next takes to come).
 // SKIP: sequences of up to that many rows are another launch's; LIMIT: and those of more.
-template <int HD, bool Q8, int QT, int RG, int TG>
+template <int HD, bool Q8, int QT, int RG, int TG, bool BLOCKS>
 struct Shape {
-    static constexpr int kRowsWg = RG * QT * kRows, kThreads = 64 * RG * TG;
+    static constexpr int NC = BLOCKS ? HD / 32 : 1;  // columns of a row
+    static constexpr int kRowsWg = RG * QT * kRows / NC;
     // waves of a SIMD: what the registers of a wave leave room for
     static constexpr int kWavesSimd = QT == 1 ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 1) : (HD <= 64 ? 3 : 2);
 };
 
-template <int HD, bool Q8, int QT, int RG, int TG>
-__global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSimd)) void k_attn(
+template <int HD, bool Q8, int QT, int RG, int TG, bool BLOCKS>
+__global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::kWavesSimd)) void k_attn(
     KvPool pool, KvAttn a, KvRows r, int group, int row_tiles, int splits, int skip, int limit) {
-    typedef Shape<HD, Q8, QT, RG, TG> S;
+    typedef Shape<HD, Q8, QT, RG, TG, BLOCKS> S;
+    static_assert(!BLOCKS || (Q8 && QT == 1 && RG == 1), "blocks as columns: one tile of few rows");
     constexpr int TB = kv_tile_bytes(Q8, HD), NU = HD / 16;
     __shared__ float sm[TG][RG][QT][kRows], sl[TG][RG][QT][kRows];
     __shared__ f4_t so[TG][RG][QT][NU][64];
@@ -473,13 +507,14 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
     if (first >= rows || rows <= skip || rows > limit) return;
     const int row0 = first + rg * QT * kRows;  // the wave's first row
     const bool busy = row0 < rows;
+    const int lr = lane & 15, lrow = lr / S::NC;  // the lane's column, and its row in a tile
     // what the wave's first and last row see
     const int least = job.sees(a, min(row0, rows - 1)), most = busy ? job.sees(a, min(row0 + QT * kRows, rows) - 1) : 0;
-    Rows<HD, Q8, QT> wave;
-    Tile<HD, Q8>(&t)[QT] = wave.t;
+    Rows<HD, Q8, BLOCKS, QT> wave;
+    auto &t = wave.t;
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
-        const int mine = row0 + j * kRows + (lane & 15), row = min(mine, rows - 1);
+        const int mine = row0 + j * kRows + lrow, row = min(mine, rows - 1);
         t[j].load_q(mine < rows ? a.q + job.qrow(row) * a.ldq + size_t(job.qhead(row)) * HD : nullptr, a.scale, lane);
         t[j].vis = job.sees(a, row);
     }
@@ -488,13 +523,13 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
     const int per = max((all + splits - 1) / splits, kLeastTiles);
     const int end = min((most + kKvTile - 1) / kKvTile, (job.split + 1) * per);
     const uint32_t *table = pool.table + size_t(job.i) * size_t(pool.table_len);
-    RawTile<HD, Q8> kr, vr;
+    RawTile<HD, Q8, BLOCKS> kr, vr;
     auto page_of = [&](int kt) __attribute__((always_inline)) {
         return kt < end ? table[kt * kKvTile >> pool.shift] : 0xffffffffu;
     };
-    auto load = [&](RawTile<HD, Q8> &x, int which, uint32_t page, int kt) __attribute__((always_inline)) {
+    auto load = [&](RawTile<HD, Q8, BLOCKS> &x, int which, uint32_t page, int kt) __attribute__((always_inline)) {
         if (page < uint32_t(pool.pages))
-            x.load(pool.pool + pool.tile_at(page, job.head, which, kt * kKvTile, TB), lane);
+            x.template load<TG == kWaves>(pool.pool + pool.tile_at(page, job.head, which, kt * kKvTile, TB), lane);
     };
     int kt = job.split * per + tg;
     bool odd = false;
@@ -544,10 +579,9 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
         for (int u = 0; u < NU; ++u) so[tg][rg][q][u][lane] = t[q].o[u];
     }
     __syncthreads();
-    const int lr = lane & 15;
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-        const int row = row0 + q * kRows + lr;
+        const int row = row0 + q * kRows + lrow;
         float m = -INFINITY, l = 0.f, f[TG];
 #pragma unroll
         for (int k = 0; k < TG; ++k) m = fmaxf(m, sm[k][rg][q][lr]);
@@ -560,6 +594,7 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG>::kWavesSim
         }
         if (row >= rows) continue;
         for (int u = tg; u < NU; u += TG) {
+            if (BLOCKS && u >> 1 != lr % S::NC) continue;  // another column's
             f4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < TG; ++k)
@@ -638,15 +673,19 @@ __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows
 // units (few rows: twice, so that sequences of different lengths even out), none under 256 tokens.
 struct Plan {
     int splits, tiles;  // shares; row tiles of the second launch
-    bool few, many;
+    bool few, many, blocks;  // blocks: the few rows' columns are blocks (q8_0)
+    int limit;               // most rows to a K/V head of a sequence of the first launch
 };
 constexpr int kFewJobs = MLG_FEW, kManyJobs = MLG_MANY;  // workgroups of a launch, about
 constexpr int kManyRows = 64;  // of a workgroup of the second launch: RG 2, and QT 2 (hd 256: RG 4, QT 1)
-Plan plan(const KvPool &p, int heads, int rows, int max_new, int max_ctx, bool uniform) {
+Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx, bool uniform) {
     Plan c;
     const long long most = (long long)max_new * (heads / p.heads);
     c.many = most > kRows;
     c.few = !c.many || !uniform;
+    const int by_block = kRows / (hd / 32);
+    c.blocks = q8 && hd > 32 && (c.many || most <= by_block);
+    c.limit = c.blocks ? by_block : kRows;
     c.tiles = int((most + kManyRows - 1) / kManyRows);
     // workgroups of the launch that has the most of the work: one for every 64 rows, at least one a sequence
     const long long of_rows = ((long long)rows * (heads / p.heads) + kManyRows - 1) / kManyRows;
@@ -659,9 +698,9 @@ Plan plan(const KvPool &p, int heads, int rows, int max_new, int max_ctx, bool u
 
 }  // namespace
 
-size_t attn_paged_scratch(const KvPool &p, int hd, int heads, int rows, int max_new, int max_ctx) {
+size_t attn_paged_scratch(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx) {
     if (p.seqs <= 0 || rows <= 0) return 0;
-    const int s = plan(p, heads, rows, max_new, max_ctx, false).splits;
+    const int s = plan(p, q8, hd, heads, rows, max_new, max_ctx, false).splits;
     return s == 1 ? 0 : size_t(rows) * size_t(heads) * size_t(s) * size_t(hd + kPartHead) * sizeof(float);
 }
 
@@ -669,19 +708,24 @@ namespace {
 template <int HD, bool Q8>
 hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx, hipStream_t st) {
     const int group = a.heads / p.heads;
-    const Plan c = plan(p, a.heads, r.rows, r.max_new, max_ctx, !r.row_off);
+    const Plan c = plan(p, Q8, HD, a.heads, r.rows, r.max_new, max_ctx, !r.row_off);
     const long long pairs = (long long)p.seqs * p.heads * c.splits, many = pairs * c.tiles;
     const long long joins = ((long long)r.rows * a.heads + kWaves - 1) / kWaves;
     if (pairs > 0x7fffffffll || many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
     constexpr int kAll = 0x7fffffff;
     if (c.many) {
         constexpr int QT = HD <= 128 ? 2 : 1, RG = kManyRows / (QT * kRows), TG = HD <= 128 ? 2 : 1;
-        hipLaunchKernelGGL((k_attn<HD, Q8, QT, RG, TG>), dim3(unsigned(many)), dim3(64 * RG * TG), 0, st, p, a, r, group,
-                           c.tiles, c.splits, c.few ? kRows : 0, kAll);
+        hipLaunchKernelGGL((k_attn<HD, Q8, QT, RG, TG, false>), dim3(unsigned(many)), dim3(64 * RG * TG), 0, st, p, a, r, group,
+                           c.tiles, c.splits, c.few ? c.limit : 0, kAll);
     }
-    if (c.few)
-        hipLaunchKernelGGL((k_attn<HD, Q8, 1, 1, kWaves>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p, a, r,
-                           group, 1, c.splits, 0, kRows);
+    if (c.few && !c.blocks)
+        hipLaunchKernelGGL((k_attn<HD, Q8, 1, 1, kWaves, false>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p, a,
+                           r, group, 1, c.splits, 0, c.limit);
+    if constexpr (Q8 && HD > 32) {
+        if (c.few && c.blocks)
+            hipLaunchKernelGGL((k_attn<HD, Q8, 1, 1, kWaves, true>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p,
+                               a, r, group, 1, c.splits, 0, c.limit);
+    }
     if (c.splits > 1)
         hipLaunchKernelGGL((k_attn_join<HD>), dim3(unsigned(joins)), dim3(64 * kWaves), 0, st, p, a, r, c.splits);
     return hipGetLastError();

@@ -103,7 +103,7 @@ struct KvAttn {
     float scale;
     float *scratch;
 };
-size_t attn_paged_scratch(const KvPool &p, int hd, int heads, int rows, int max_new, int max_ctx);
+size_t attn_paged_scratch(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx);
 hipError_t attn_paged(const KvPool &p, bool q8, int hd, const KvAttn &a, const KvRows &r, int max_ctx, hipStream_t st);
 
 }  // namespace mlg
