@@ -264,9 +264,15 @@ struct Tile {
     }
     // Whether it takes a row's p past 2^15.
     __device__ __forceinline__ bool behind(float t) const { return t > m + kPSlack; }
-    // m, l and out follow it.
-    __device__ __forceinline__ void follow(float t) {
-        const float mn = fmaxf(m, t), al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    // m, l and out follow it, and (q8_0) the exponent x.
+    __device__ __forceinline__ void follow(float t, int x) {
+        const float mn = fmaxf(m, t);
+        float al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        if constexpr (Q8) {
+            const int en = max(e, x);
+            al = ldexpf(al, max(e - en, -126));
+            e = en;
+        }
         l *= al;
 #pragma unroll
         for (int u = 0; u < NU; ++u) o[u] *= al;
@@ -341,10 +347,17 @@ struct Rows {
             }
     }
 
-    // m follows the tile's scores where a row's p would grow too large.
-    __device__ __forceinline__ void follow(const float (&s)[QT][8]) {
+    // m follows the tile's scores where a row's p would grow too large. q8_0: e likewise a larger scale of
+    // V than any before, so that p times a scale stays within f16's range (below 2^16) and keeps its bits
+    // whatever the scales' size.
+    __device__ __forceinline__ void follow(const float (&s)[QT][8], const Raw &v) {
         float top[QT];
+        int x = 0;
         bool behind = false;
+        if constexpr (Q8) {
+            x = v.top_exponent();
+            behind = x > t[0].e;
+        }
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
             top[q] = t[q].top(s[q]);
@@ -352,24 +365,7 @@ struct Rows {
         }
         if (__any(behind)) {  // wave-uniform
 #pragma unroll
-            for (int q = 0; q < QT; ++q) t[q].follow(top[q]);
-        }
-    }
-
-    // q8_0: l and out follow a larger scale of V than any before, so that p times a scale stays within
-    // f16's range (below 2^16) and keeps its bits whatever the scales' size.
-    __device__ __forceinline__ void fit(const Raw &v) {
-        const int x = v.top_exponent();
-        if (__any(x > t[0].e)) {
-            const int en = max(x, t[0].e);
-            const float f = ldexpf(1.f, max(t[0].e - en, -126));
-#pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                t[q].l *= f;
-#pragma unroll
-                for (int u = 0; u < NU; ++u) t[q].o[u] *= f;
-                t[q].e = en;
-            }
+            for (int q = 0; q < QT; ++q) t[q].follow(top[q], x);
         }
     }
 
@@ -377,7 +373,6 @@ struct Rows {
     template <bool MASKED>
     __device__ __forceinline__ void values(const Raw &v, float (&s)[QT][8]) {
         if constexpr (Q8) {
-            fit(v);
 #pragma unroll
             for (int q = 0; q < QT; ++q) t[q].probs(s[q]);
             auto scaled = [&](int q, int c, h8_t &ph, h8_t &pl) __attribute__((always_inline)) {
@@ -527,9 +522,12 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
     auto page_of = [&](int kt) __attribute__((always_inline)) {
         return kt < end ? table[kt * kKvTile >> pool.shift] : 0xffffffffu;
     };
+    // Always loads: where there is no such tile, or its page does not exist, from the pool's first one,
+    // and the result is not used. (Loads that may not happen would have to be waited for at once.)
     auto load = [&](RawTile<HD, Q8, BLOCKS> &x, int which, uint32_t page, int kt) __attribute__((always_inline)) {
-        if (page < uint32_t(pool.pages))
-            x.template load<TG == kWaves>(pool.pool + pool.tile_at(page, job.head, which, kt * kKvTile, TB), lane);
+        const bool there = page < uint32_t(pool.pages);
+        const size_t at = pool.tile_at(there ? page : 0u, there ? job.head : 0, which, there ? kt * kKvTile : 0, TB);
+        x.template load<TG == kWaves>(pool.pool + at, lane);
     };
     int kt = job.split * per + tg;
     bool odd = false;
@@ -550,7 +548,7 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
                 for (int q = 0; q < QT; ++q) t[q].hide(p[q], tok0);
                 odd |= vr.cut(s.ctx - tok0 - 8 * (lane >> 4));
             }
-            wave.follow(p);
+            wave.follow(p, vr);
             wave.template values<kMasked>(vr, p);
         }
         load(vr, 1, next, kt + TG);
