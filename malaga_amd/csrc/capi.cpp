@@ -168,6 +168,9 @@ int check_kv(const mlg_kv_cache *c, std::initializer_list<const void *> arrays, 
         return set_err(MLG_ERR_UNSUPPORTED, w + ": head size and page of 32, 64, 128 or 256");
     if (int64_t(c->page) * c->table_len > 0x7fffffff)
         return set_err(MLG_ERR_INVALID, w + ": more than 2^31 - 1 tokens in a table row");
+    if (int64_t(c->heads) * 2 * (c->page / mlg::kKvTile) * mlg::kv_tile_bytes(c->type == MLG_Q8_0, c->head_size) >
+        0xffffffffll)
+        return set_err(MLG_ERR_INVALID, w + ": a page of 2^32 bytes or more");
     if (int64_t(heads) * c->head_size > 0x7fffffff) return set_err(MLG_ERR_INVALID, w + ": too many heads");
     if (!row_off && int64_t(c->seqs) * max_new > rows)
         return set_err(MLG_ERR_INVALID, w + ": fewer rows than max_new for every sequence");

@@ -319,25 +319,27 @@ struct Rows {
 
     // The lane's 8 products (tokens 8 g .. 8 g + 7 of the tile) for its row of each tile, not yet times qf.
     __device__ __forceinline__ void scores(const Raw &k, float (&s)[QT][8]) const {
+        // lo of q first; products that wait for each other lie 2 QT apart
+        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
         f4_t acc[QT][2];
+        static_for<0, NC>([&](auto c_) __attribute__((always_inline)) {
+            constexpr int c = decltype(c_)::value;
+            constexpr bool kOwn = Q8 && !BLOCKS;  // a sum of its own for each block, for its scales
+            const h8_t kf[2] = {k.frag(2 * c), k.frag(2 * c + 1)};
+            f4_t x[QT][2];
 #pragma unroll
-        for (int q = 0; q < QT; ++q) acc[q][0] = acc[q][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 2 * QT; ++i)
+                x[i >> 1][i & 1] = mfma(kf[i & 1], t[i >> 1].ql[c], kOwn || c == 0 ? zero : acc[i >> 1][i & 1]);
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+            for (int i = 0; i < 2 * QT; ++i) x[i >> 1][i & 1] = mfma(kf[i & 1], t[i >> 1].qh[c], x[i >> 1][i & 1]);
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const h8_t kf = k.frag(2 * c + b);
+            for (int q = 0; q < QT; ++q)
 #pragma unroll
-                for (int q = 0; q < QT; ++q) {
-                    if constexpr (Q8 && !BLOCKS) {
-                        const f4_t x = mfma(kf, t[q].qh[c], mfma(kf, t[q].ql[c], f4_t{0.f, 0.f, 0.f, 0.f}));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[q][b][i] = fmaf(x[i], k.scale(c, 4 * b + i), acc[q][b][i]);
-                    } else {
-                        acc[q][b] = mfma(kf, t[q].qh[c], mfma(kf, t[q].ql[c], acc[q][b]));
-                    }
+                for (int n = 0; n < 8; ++n) {
+                    const float z = x[q][n >> 2][n & 3];
+                    acc[q][n >> 2][n & 3] = !kOwn ? z : fmaf(z, k.scale(c, n), c == 0 ? 0.f : acc[q][n >> 2][n & 3]);
                 }
-            }
+        });
 #pragma unroll
         for (int q = 0; q < QT; ++q)
 #pragma unroll
@@ -405,12 +407,12 @@ struct Rows {
                 t[q].probs(s[q]);
                 h8_t ph, pl;
                 split8(s[q], ph, pl);
-                t[q].l = mfma(one, ph, mfma(one, pl, t[q].l));
+                t[q].l = mfma(one, pl, t[q].l);
 #pragma unroll
-                for (int u = 0; u < NU; ++u) {
-                    const h8_t vf = v.frag(u);
-                    t[q].o[u] = mfma(vf, ph, mfma(vf, pl, t[q].o[u]));
-                }
+                for (int u = 0; u < NU; ++u) t[q].o[u] = mfma(v.frag(u), pl, t[q].o[u]);
+                t[q].l = mfma(one, ph, t[q].l);
+#pragma unroll
+                for (int u = 0; u < NU; ++u) t[q].o[u] = mfma(v.frag(u), ph, t[q].o[u]);
             }
         }
     }
@@ -524,16 +526,19 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
     };
     // Always loads: where there is no such tile, or its page does not exist, from the pool's first one,
     // and the result is not used. (Loads that may not happen would have to be waited for at once.)
-    auto load = [&](RawTile<HD, Q8, BLOCKS> &x, int which, uint32_t page, int kt) __attribute__((always_inline)) {
+    const uint32_t in_page = (1u << (pool.shift - 5)) - 1u, to_v = (in_page + 1u) * TB;
+    const uint32_t head_at = uint32_t(job.head) * 2u * to_v, page_bytes = uint32_t(pool.heads) * 2u * to_v;
+    auto tile_of = [&](uint32_t page, int kt) __attribute__((always_inline)) {
         const bool there = page < uint32_t(pool.pages);
-        const size_t at = pool.tile_at(there ? page : 0u, there ? job.head : 0, which, there ? kt * kKvTile : 0, TB);
-        x.template load<TG == kWaves>(pool.pool + at, lane);
+        return pool.pool + size_t(there ? page : 0u) * page_bytes + (there ? head_at + (uint32_t(kt) & in_page) * TB : 0u);
     };
     int kt = job.split * per + tg;
     bool odd = false;
     uint32_t page = page_of(kt), next = page_of(kt + TG);
-    load(kr, 0, page, kt);
-    load(vr, 1, page, kt);
+    constexpr bool kOnce = TG == kWaves;
+    const uint8_t *at = tile_of(page, kt);
+    kr.template load<kOnce>(at, lane);
+    vr.template load<kOnce>(at + to_v, lane);
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
         const int tok0 = kt * kKvTile;
@@ -541,7 +546,8 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
         float p[QT][8];
         if (there) wave.scores(kr, p);
         else if (r.bad && lane == 0) *r.bad = 1u;  // its tokens are not there
-        load(kr, 0, next, kt + TG);
+        at = tile_of(next, kt + TG);
+        kr.template load<kOnce>(at, lane);
         if (there) {
             if constexpr (kMasked) {
 #pragma unroll
@@ -551,7 +557,7 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
             wave.follow(p, vr);
             wave.template values<kMasked>(vr, p);
         }
-        load(vr, 1, next, kt + TG);
+        vr.template load<kOnce>(at + to_v, lane);
         page = next;
         next = page_of(kt + 2 * TG);
     };
@@ -564,7 +570,7 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
             if (const uint32_t id = page_of(kt); id < uint32_t(pool.pages))
 #pragma unroll
                 for (int q = 0; q < QT; ++q)
-                    t[q].not_finite(pool.pool + pool.tile_at(id, job.head, 1, kt * kKvTile, TB), kt * kKvTile, s.ctx);
+                    t[q].not_finite(tile_of(id, kt) + to_v, kt * kKvTile, s.ctx);
     // the results of the waves with the same rows meet in LDS
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
