@@ -20,10 +20,6 @@
 namespace mlg {
 namespace {
 
-#ifndef MLG_FEW
-#define MLG_FEW 2048
-#define MLG_MANY 2048
-#endif
 constexpr int kRows = 16;        // rows of a query tile (columns of the matrix products)
 constexpr int kWaves = 4;        // waves of a workgroup
 // p = 2^(s - m): m is the running maximum of the scores (log2 units) less kPShift, and follows a larger
@@ -113,6 +109,12 @@ struct RawTile {
             for (int c = 0; c < ND; ++c)
                 d[c] = at(tile + kv_scale_byte(HD, 8 * (lane >> 4), BLOCKS ? (lane & 15) % NC : c));
         }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) a[i] = u4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < ND; ++i) d[i] = u4_t{0u, 0u, 0u, 0u};
     }
     // As a matrix operand: K's product b of dims 32 c .. at 2 c + b, V's dims 16 u .. at u.
     __device__ __forceinline__ h8_t frag(int i) const {
@@ -474,7 +476,8 @@ struct Shape {
     static constexpr int NC = BLOCKS ? HD / 32 : 1;  // columns of a row
     static constexpr int kRowsWg = RG * QT * kRows / NC;
     // waves of a SIMD: what the registers of a wave leave room for
-    static constexpr int kWavesSimd = QT == 1 ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 1) : (HD <= 64 ? 3 : 2);
+    static constexpr int kWavesSimd =
+        QT == 1 ? (HD <= 64 ? 4 : HD <= 128 ? (Q8 ? 3 : 2) : 1) : HD <= 64 && QT == 2 ? 3 : 2;
 };
 
 template <int HD, bool Q8, int QT, int RG, int TG, bool BLOCKS>
@@ -542,21 +545,23 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
         const int tok0 = kt * kKvTile;
-        const bool there = page < uint32_t(pool.pages);
         float p[QT][8];
-        if (there) wave.scores(kr, p);
-        else if (r.bad && lane == 0) *r.bad = 1u;  // its tokens are not there
+        wave.scores(kr, p);
         at = tile_of(next, kt + TG);
         kr.template load<kOnce>(at, lane);
-        if (there) {
-            if constexpr (kMasked) {
+        if (page >= uint32_t(pool.pages)) {  // its tokens are not there
+            if (r.bad && lane == 0) *r.bad = 1u;
 #pragma unroll
-                for (int q = 0; q < QT; ++q) t[q].hide(p[q], tok0);
-                odd |= vr.cut(s.ctx - tok0 - 8 * (lane >> 4));
-            }
-            wave.follow(p, vr);
-            wave.template values<kMasked>(vr, p);
+            for (int q = 0; q < QT; ++q) t[q].hide(p[q], 0x7fffffe0);
+            vr.clear();
         }
+        if constexpr (kMasked) {
+#pragma unroll
+            for (int q = 0; q < QT; ++q) t[q].hide(p[q], tok0);
+            odd |= vr.cut(s.ctx - tok0 - 8 * (lane >> 4));
+        }
+        wave.follow(p, vr);
+        wave.template values<kMasked>(vr, p);
         vr.template load<kOnce>(at + to_v, lane);
         page = next;
         next = page_of(kt + 2 * TG);
@@ -608,27 +613,72 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
     }
 }
 
-// The splits of a row joined in their order. A wave per (row, head): lane k weighs split k, all of their
-// m and l read at once; then the outs, 16 bytes a lane, as many splits at a time as a wave has lanes for.
+// Whether some sequence has the row, for the 64 / LANES rows of a wave at once (each the same in its
+// LANES neighbouring lanes): a row that is none's, or past max_new of its own, is left alone.
+template <int LANES>
+__device__ __forceinline__ bool is_a_row(const KvPool &pool, const KvRows &r, size_t qrow) {
+    const int lane = threadIdx.x & 63;
+    if (!r.row_off) return qrow < size_t(pool.seqs) * size_t(r.max_new);
+    const uint64_t mine = (LANES == 64 ? ~0ull : (1ull << LANES) - 1ull) << (lane / LANES * LANES);
+    bool found = false;
+    for (int i0 = 0; i0 < pool.seqs; i0 += LANES) {  // wave-uniform
+        const int i = i0 + lane % LANES;
+        bool in = false;
+        if (i < pool.seqs) {
+            const KvSeq s = kv_seq(pool, r, i);
+            in = qrow >= size_t(s.r0) && qrow < size_t(s.r0) + size_t(s.n);
+        }
+        found |= (__ballot(in) & mine) != 0ull;
+    }
+    return found;
+}
+
+// The splits of a row joined in their order, a few of them: HD / 4 lanes to a (row, head).
+template <int HD>
+__global__ __launch_bounds__(256) void k_attn_join_few(KvPool pool, KvAttn a, KvRows r, int splits) {
+    constexpr int LANES = HD / 4, PART = HD + kPartHead;
+    const size_t job = (size_t(blockIdx.x) * 256 + threadIdx.x) / LANES, qrow = job / size_t(a.heads);
+    const int head = int(job % size_t(a.heads)), lane = threadIdx.x % LANES;
+    if (!is_a_row<LANES>(pool, r, qrow) || qrow >= size_t(r.rows)) return;
+    const float *part = a.scratch + job * size_t(splits) * size_t(PART);
+    float m = -INFINITY, l = 0.f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < splits; k0 += 4) {
+        float mk[4], lk[4];
+        f4_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float *pk = part + size_t(min(k0 + j, splits - 1)) * PART;
+            mk[j] = k0 + j < splits ? pk[0] : -INFINITY;
+            lk[j] = k0 + j < splits ? pk[1] : 0.f;
+            x[j] = *reinterpret_cast<const f4_t *>(pk + kPartHead + 4 * lane);  // not used where there is none
+        }
+        const float mn = fmaxf(fmaxf(fmaxf(mk[0], mk[1]), fmaxf(mk[2], mk[3])), m);
+        const float down = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l = l == 0.f ? 0.f : l * down;
+        o *= down;
+        m = mn;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (lk[j] == 0.f) continue;  // a split that saw no token adds nothing (and has no out)
+            const float f = mk[j] == m ? 1.f : __builtin_amdgcn_exp2f(mk[j] - m);
+            l += f * lk[j];
+            o += x[j] * f;
+        }
+    }
+    const f4_t y = l == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : o / l;
+    *reinterpret_cast<f4_t *>(a.out + qrow * a.ldo + size_t(head) * HD + 4 * lane) = y;
+}
+
+// The same for many: a wave to a (row, head). Lane k weighs split k, all of their m and l read at once;
+// then the outs, 16 bytes a lane, as many splits at a time as a wave has lanes for.
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows r, int splits) {
     constexpr int LANES = HD / 4, AT = 64 / LANES, PART = HD + kPartHead;  // lanes of an out; outs at a time
     const int lane = threadIdx.x & 63;
     const size_t job = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6), qrow = job / size_t(a.heads);
     const int head = int(job % size_t(a.heads));
-    if (qrow >= size_t(r.rows)) return;
-    // the sequence that has the row; a row that is none's, or past max_new of its own, is left alone
-    bool mine = false;
-    for (int i0 = 0; i0 < pool.seqs && !mine; i0 += 64) {  // wave-uniform
-        const int i = i0 + lane;
-        bool in = false;
-        if (i < pool.seqs) {
-            const KvSeq s = kv_seq(pool, r, i);
-            in = qrow >= size_t(s.r0) && qrow < size_t(s.r0) + size_t(s.n);
-        }
-        mine = __any(in);
-    }
-    if (!mine) return;
+    if (!is_a_row<64>(pool, r, qrow) || qrow >= size_t(r.rows)) return;
     const float *part = a.scratch + (qrow * size_t(a.heads) + size_t(head)) * size_t(splits) * size_t(PART);
     float m = -INFINITY, l = 0.f;
     f4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -680,7 +730,8 @@ struct Plan {
     bool few, many, blocks;  // blocks: the few rows' columns are blocks (q8_0)
     int limit;               // most rows to a K/V head of a sequence of the first launch
 };
-constexpr int kFewJobs = MLG_FEW, kManyJobs = MLG_MANY;  // workgroups of a launch, about
+constexpr int kFewSplits = 8;
+constexpr int kFewJobs = 2048, kManyJobs = 1536;  // workgroups of a launch, about
 constexpr int kManyRows = 64;  // of a workgroup of the second launch: RG 2, and QT 2 (hd 256: RG 4, QT 1)
 Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx, bool uniform) {
     Plan c;
@@ -714,7 +765,9 @@ hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx
     const int group = a.heads / p.heads;
     const Plan c = plan(p, Q8, HD, a.heads, r.rows, r.max_new, max_ctx, !r.row_off);
     const long long pairs = (long long)p.seqs * p.heads * c.splits, many = pairs * c.tiles;
-    const long long joins = ((long long)r.rows * a.heads + kWaves - 1) / kWaves;
+    const bool few = c.splits <= kFewSplits;
+    const int per = few ? 256 / (HD / 4) : kWaves;  // (row, head)s of a workgroup of the join
+    const long long joins = ((long long)r.rows * a.heads + per - 1) / per;
     if (pairs > 0x7fffffffll || many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
     constexpr int kAll = 0x7fffffff;
     if (c.many) {
@@ -730,8 +783,10 @@ hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx
             hipLaunchKernelGGL((k_attn<HD, Q8, 1, 1, kWaves, true>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p,
                                a, r, group, 1, c.splits, 0, c.limit);
     }
-    if (c.splits > 1)
-        hipLaunchKernelGGL((k_attn_join<HD>), dim3(unsigned(joins)), dim3(64 * kWaves), 0, st, p, a, r, c.splits);
+    if (c.splits > 1 && few)
+        hipLaunchKernelGGL((k_attn_join_few<HD>), dim3(unsigned(joins)), dim3(256), 0, st, p, a, r, c.splits);
+    if (c.splits > 1 && !few)
+        hipLaunchKernelGGL((k_attn_join<HD>), dim3(unsigned(joins)), dim3(256), 0, st, p, a, r, c.splits);
     return hipGetLastError();
 }
 }  // namespace
