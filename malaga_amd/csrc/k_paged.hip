@@ -1,10 +1,10 @@
 // Writing and reading the paged K/V cache (paged_kv.hpp has the layout).
 //
-// Both kernels give a wave one 1 KB piece of a tile (q8_0: with its two halves), lane l to the
-// piece's bytes 16 l .. 16 l + 15, so the cache's side of the copy is whole lines: 4 KB per tile
-// at hd 64 f16. The f32 side is then 128-byte runs of 16 rows for K (a lane's 8 dims of one token)
-// and 64-byte runs for V (a lane's one dim of 8 tokens). A workgroup of 4 waves takes a tile's K and
-// V of one head.
+// Both are copies: bytes alone bound them. A workgroup of 4 waves takes a tile's K and V of one head, a
+// wave a block of 32 dims of either: 4 KB of f32 rows in runs of 128 bytes, and of the cache the 2 KB
+// (f16) or 1 KB (q8_0) that lie together. K: a lane has 8 dims of two tokens, V: two dims of 8 tokens,
+// the operands that the attention reads. The f32 rows pass the caches by (non-temporal): nothing reads
+// them again from there soon, and what the cache takes may stay.
 #include "device.hpp"
 #include "paged_kv.hpp"
 
@@ -44,142 +44,178 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
     return uint32_t(__half_as_ushort(__float2half_rn(a))) | uint32_t(__half_as_ushort(__float2half_rn(b))) << 16;
 }
 
-// A q8_0 block's scale and its inverse from max |x| of its 32 values, and whether every one of them
-// is finite: d = amax / 127 and 1 / d in f32, as the GGUF codec computes them. A block with a value
-// that is not finite is stored as NaN (d), so that it reads back as NaN instead of a wrong number.
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+
+// A q8_0 block's scale and its inverse from max |x| of its 32 values, inf where one of them is not
+// finite: d = amax / 127 and 1 / d in f32, as the GGUF codec computes them. A block with a value that
+// is not finite is stored as NaN (d), so that it reads back as NaN instead of a wrong number.
 struct Q8Scale {
     float inv;
-    uint16_t d;
+    uint32_t d;  // f16 bits
 };
-__device__ __forceinline__ Q8Scale q8_scale(float amax, bool finite) {
+__device__ __forceinline__ Q8Scale q8_scale(float amax) {
     Q8Scale s;
+    const bool finite = amax < INFINITY;
     const float d = __fdiv_rn(amax, 127.f);
     s.inv = d > 0.f && finite ? __fdiv_rn(1.f, d) : 0.f;
     if (!(s.inv < INFINITY)) s.inv = 0.f;  // d below 2^-128: it is stored as 0 whatever q says
-    s.d = finite ? __half_as_ushort(__float2half_rn(d)) : uint16_t(0x7e00u);
+    s.d = finite ? __half_as_ushort(__float2half_rn(d)) : 0x7e00u;
     return s;
 }
-__device__ __forceinline__ uint32_t q8_value(float x, const Q8Scale &s) {
-    // round half away from zero; a value that is not finite has inv = 0 and its product dropped
-    const float y = s.inv > 0.f ? roundf(__fmul_rn(x, s.inv)) : 0.f;
-    return uint32_t(int(fminf(fmaxf(y, -127.f), 127.f))) & 0xffu;
+// Four values as int8: x / d rounded half away from zero, |x| inv <= 127 + 2^-16. The largest number
+// below 0.5 added with x's sign rounds to the next integer exactly where the half does (at y + 0.5 - 2^-25
+// a tie goes to the even number, which is the integer), and leaves all that is below the half below it.
+// inf times inv = 0 is NaN, which converts to 0.
+__device__ __forceinline__ uint32_t q8_four(float a, float b, float c, float d, float inv) {
+    auto one = [&](float x) __attribute__((always_inline)) {
+        const float y = __fmul_rn(x, inv);
+        return uint32_t(int(__fadd_rn(y, copysignf(0x1.fffffep-2f, y))));
+    };
+    const uint32_t lo = __builtin_amdgcn_perm(one(b), one(a), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(one(d), one(c), 0x04000c0cu);
+    return lo | hi;
 }
+__device__ __forceinline__ float largest(float m, float x) {  // inf for a value that is not finite
+    return fabsf(x) < INFINITY ? fmaxf(m, fabsf(x)) : INFINITY;
+}
+// v of lane N of the lane's 16.
+template <int N>
+__device__ __forceinline__ float of_lane16(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x150 + N, 0xf, 0xf, true));
+}
+
+// K rows: lane 16 g + r has dims 8 g .. 8 g + 7 of a token's 32, in memory 16-byte chunks 2 g and 2 g + 1.
+// A load or store of chunk 2 g alone would take every other 16 bytes; instead the first of the two takes
+// chunks 0 .. 3, lane g's at chunk_of(g), the second 4 .. 7, and the halves of the wave trade places.
+__device__ __forceinline__ int chunk_of(int g) { return (g & 1) * 2 + (g >> 1); }
+__device__ __forceinline__ void trade(f4_t &a, f4_t &b) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a[n]), __float_as_uint(b[n]), false, false);
+        a[n] = __uint_as_float(r[0]);
+        b[n] = __uint_as_float(r[1]);
+    }
+}
+
+__device__ __forceinline__ float i8_of(uint32_t w, int n) { return float(int(w << (24 - 8 * n)) >> 24); }
 
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void k_kv_write(KvPool p, const float *k, size_t ldk, const float *v, size_t ldv,
                                                   KvRows r, int tiles) {
     const TileJob j = tile_job(p, r, tiles);
     if (!j.have || j.page == 0xffffffffu) return;
-    constexpr int TB = kv_tile_bytes(Q8, HD), NC = HD / 32, NP = Q8 ? NC : 2 * NC;
+    constexpr int TB = kv_tile_bytes(Q8, HD), NC = HD / 32;
     const int lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-    for (int w = int(threadIdx.x >> 6); w < 2 * NP; w += 4) {  // wave-uniform
-        const int which = w >= NP, pc = which ? w - NP : w;
+    for (int w = int(threadIdx.x >> 6); w < 2 * NC; w += 4) {  // wave-uniform
+        const int which = w >= NC, c = which ? w - NC : w;
         uint8_t *tile = p.pool + p.tile_at(j.page, j.head, which, j.base, TB);
-        // row of the token at position pos: j.s.r0 + pos - j.first
         if (!which) {
-            constexpr int NB = Q8 ? 2 : 1;  // tokens of this lane
-            const int c = Q8 ? pc : pc >> 1;
-            float x[NB][8];
-            bool in[NB];
+            // row of the token at position pos: j.s.r0 + pos - j.first
+            f4_t x[2][2];
+            bool in[2];
+            const int t0 = 8 * (lr >> 2) + (lr & 3);
 #pragma unroll
-            for (int e = 0; e < NB; ++e) {
-                const int t = 8 * (lr >> 2) + 4 * (Q8 ? e : pc & 1) + (lr & 3), pos = j.base + t;
-                in[e] = pos >= j.first && pos < j.s.ctx;
-                if (in[e]) {
-                    const float *src = k + size_t(j.s.r0 + pos - j.first) * ldk + size_t(j.head) * HD + 32 * c + 8 * g;
-                    const float4 a = ld4(src, 0), b = ld4(src, 1);
-                    x[e][0] = a.x, x[e][1] = a.y, x[e][2] = a.z, x[e][3] = a.w;
-                    x[e][4] = b.x, x[e][5] = b.y, x[e][6] = b.z, x[e][7] = b.w;
-                } else {
+            for (int b = 0; b < 2; ++b) {
+                const int pos = j.base + t0 + 4 * b;
+                in[b] = pos >= j.first && pos < j.s.ctx;
+                const f4_t *src = reinterpret_cast<const f4_t *>(k + size_t(j.s.r0 + (in[b] ? pos - j.first : 0)) * ldk +
+                                                                 size_t(j.head) * HD + 32 * c) + chunk_of(g);
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) x[e][n] = 0.f;
-                }
+                for (int h = 0; h < 2; ++h)
+                    x[b][h] = in[b] ? __builtin_nontemporal_load(src + 4 * h) : f4_t{0.f, 0.f, 0.f, 0.f};
             }
-            if constexpr (!Q8) {
-                if (in[0])
-                    *reinterpret_cast<uint4 *>(tile + (pc * 64 + lane) * 16) =
-                        make_uint4(pack_h2(x[0][0], x[0][1]), pack_h2(x[0][2], x[0][3]), pack_h2(x[0][4], x[0][5]),
-                                   pack_h2(x[0][6], x[0][7]));
-            } else {
 #pragma unroll
-                for (int e = 0; e < NB; ++e) {
+            for (int b = 0; b < 2; ++b) trade(x[b][0], x[b][1]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if constexpr (!Q8) {
+                    if (in[b])
+                        *reinterpret_cast<u4_t *>(tile + ((2 * c + b) * 64 + lane) * 16) =
+                            u4_t{pack_h2(x[b][0][0], x[b][0][1]), pack_h2(x[b][0][2], x[b][0][3]),
+                                 pack_h2(x[b][1][0], x[b][1][1]), pack_h2(x[b][1][2], x[b][1][3])};
+                } else {
                     float amax = 0.f;
-                    bool bad = false;
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        amax = fmaxf(amax, fabsf(x[e][n]));
-                        bad |= !(fabsf(x[e][n]) < INFINITY);
-                    }
+                    for (int n = 0; n < 8; ++n) amax = largest(amax, x[b][n >> 2][n & 3]);
                     // the block's four k-groups: lanes lr, 16 + lr, 32 + lr, 48 + lr
-                    if (bad) amax = INFINITY;
                     amax = fmaxf(amax, __shfl_xor(amax, 16));
                     amax = fmaxf(amax, __shfl_xor(amax, 32));
-                    const Q8Scale sc = q8_scale(amax, amax < INFINITY);
-                    uint32_t q[2] = {0u, 0u};
+                    const Q8Scale sc = q8_scale(amax);
+                    u2_t q;
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) q[n >> 2] |= q8_value(x[e][n], sc) << (8 * (n & 3));
-                    if (in[e]) {
-                        *reinterpret_cast<uint2 *>(tile + (pc * 64 + lane) * 16 + 8 * e) = make_uint2(q[0], q[1]);
-                        const int t = 8 * (lr >> 2) + 4 * e + (lr & 3);
-                        if (g == 0) *reinterpret_cast<uint16_t *>(tile + kv_scale_byte(HD, t, c)) = sc.d;
+                    for (int h = 0; h < 2; ++h) q[h] = q8_four(x[b][h][0], x[b][h][1], x[b][h][2], x[b][h][3], sc.inv);
+                    if (in[b]) {
+                        *reinterpret_cast<u2_t *>(tile + (c * 64 + lane) * 16 + 8 * b) = q;
+                        if (g == 0) *reinterpret_cast<uint16_t *>(tile + kv_scale_byte(HD, t0 + 4 * b, c)) = uint16_t(sc.d);
                     }
                 }
             }
         } else {
-            constexpr int NU = Q8 ? 2 : 1;  // dims of this lane
-            // its 8 tokens 8 g .. 8 g + 7: which are new, lo <= n < hi
+            // dims 32 c + 2 lr + 0, 1 of tokens 8 g .. 8 g + 7: which are new, lo <= n < hi
             const int lo = max(0, j.first - j.base - 8 * g), hi = min(8, j.s.ctx - j.base - 8 * g);
-            float x[NU][8];
+            f2_t x[8];
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const bool in = n >= lo && n < hi;
-                const float *src = v + size_t(in ? j.s.r0 + j.base + 8 * g + n - j.first : j.s.r0) * ldv +
-                                   size_t(j.head) * HD + 16 * NU * pc + lr;
-#pragma unroll
-                for (int u = 0; u < NU; ++u) x[u][n] = in ? src[16 * u] : 0.f;
+                const f2_t *src = reinterpret_cast<const f2_t *>(
+                    v + size_t(in ? j.s.r0 + j.base + 8 * g + n - j.first : j.s.r0) * ldv + size_t(j.head) * HD +
+                    32 * c + 2 * lr);
+                x[n] = in ? __builtin_nontemporal_load(src) : f2_t{0.f, 0.f};
             }
+            const bool all = lo == 0 && hi == 8;
             if constexpr (!Q8) {
-                uint32_t h[4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) h[n] = pack_h2(x[0][2 * n], x[0][2 * n + 1]);
-                uint8_t *at = tile + (pc * 64 + lane) * 16;
-                if (lo == 0 && hi == 8) {
-                    *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-                } else {
+                for (int e = 0; e < 2; ++e) {
+                    u4_t h;
 #pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                        if (n >= lo && n < hi)
-                            reinterpret_cast<uint16_t *>(at)[n] = uint16_t(h[n >> 1] >> (16 * (n & 1)));
+                    for (int n = 0; n < 4; ++n) h[n] = pack_h2(x[2 * n][e], x[2 * n + 1][e]);
+                    uint8_t *at = tile + ((2 * c + (lr >> 3)) * 64 + g * 16 + (2 * lr & 15) + e) * 16;
+                    if (all) {
+                        *reinterpret_cast<u4_t *>(at) = h;
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+                            if (n >= lo && n < hi)
+                                reinterpret_cast<uint16_t *>(at)[n] = uint16_t(h[n >> 1] >> (16 * (n & 1)));
+                    }
                 }
             } else {
-                uint32_t q[2][2] = {{0u, 0u}, {0u, 0u}};
-                uint16_t d[8];
+                // lane n of the 16 (and n + 8) computes the scale of token n, the others take it from there
+                float own = 0.f;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    float amax = fmaxf(fabsf(x[0][n]), fabsf(x[1][n]));
-                    if (!(fabsf(x[0][n]) < INFINITY) || !(fabsf(x[1][n]) < INFINITY)) amax = INFINITY;
-                    amax = group_reduce(amax, 4, OpMax{});  // the block's 32 dims: 16 lanes
-                    const Q8Scale sc = q8_scale(amax, amax < INFINITY);
-                    d[n] = sc.d;
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) q[u][n >> 2] |= q8_value(x[u][n], sc) << (8 * (n & 3));
+                    // the block's 32 dims: 16 lanes
+                    const float amax = group_reduce(largest(largest(0.f, x[n][0]), x[n][1]), 4, OpMax{});
+                    own = (lr & 7) == n ? amax : own;
                 }
-                uint8_t *at = tile + (pc * 64 + lane) * 16, *sd = tile + kv_scale_byte(HD, 8 * g, pc);
-                if (lo == 0 && hi == 8) {
-                    *reinterpret_cast<uint4 *>(at) = make_uint4(q[0][0], q[0][1], q[1][0], q[1][1]);
-                    if (lr == 0)
-                        *reinterpret_cast<uint4 *>(sd) =
-                            make_uint4(d[0] | uint32_t(d[1]) << 16, d[2] | uint32_t(d[3]) << 16,
-                                       d[4] | uint32_t(d[5]) << 16, d[6] | uint32_t(d[7]) << 16);
-                } else {
+                const Q8Scale sc = q8_scale(own);
+                float inv[8];
+                static_for<0, 8>([&](auto n) __attribute__((always_inline)) {
+                    inv[decltype(n)::value] = of_lane16<decltype(n)::value>(sc.inv);
+                });
 #pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                        if (n >= lo && n < hi) {
-                            at[n] = uint8_t(q[0][n >> 2] >> (8 * (n & 3)));
-                            at[8 + n] = uint8_t(q[1][n >> 2] >> (8 * (n & 3)));
-                            if (lr == 0) reinterpret_cast<uint16_t *>(sd)[n] = d[n];
-                        }
+                for (int e = 0; e < 2; ++e) {
+                    u2_t q;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float y[4];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) y[n] = __fmul_rn(x[4 * h + n][e], inv[4 * h + n]);
+                        q[h] = q8_four(y[0], y[1], y[2], y[3], 1.f);
+                    }
+                    uint8_t *at = tile + (c * 64 + g * 16 + (2 * lr & 15) + e) * 16 + 8 * (lr >> 3);
+                    if (all) {
+                        *reinterpret_cast<u2_t *>(at) = q;
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+                            if (n >= lo && n < hi) at[n] = uint8_t(q[n >> 2] >> (8 * (n & 3)));
+                    }
                 }
+                if (lr >= lo && lr < hi)
+                    *reinterpret_cast<uint16_t *>(tile + kv_scale_byte(HD, 8 * g + lr, c)) = uint16_t(sc.d);
             }
         }
     }
@@ -189,7 +225,7 @@ template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void k_kv_read(KvPool p, float *k, size_t ldk, float *v, size_t ldv, KvRows r,
                                                  int tiles) {
     const TileJob j = tile_job(p, r, tiles);
-    constexpr int TB = kv_tile_bytes(Q8, HD), NC = HD / 32, NP = Q8 ? NC : 2 * NC;
+    constexpr int TB = kv_tile_bytes(Q8, HD), NC = HD / 32;
     const int lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
     if (!j.have || j.page == 0xffffffffu) {  // no place to read: rows of zeros
         const bool lost = j.have || !j.s.ok || j.first < 0;
@@ -205,50 +241,63 @@ __global__ __launch_bounds__(256) void k_kv_read(KvPool p, float *k, size_t ldk,
         }
         return;
     }
-    for (int w = int(threadIdx.x >> 6); w < 2 * NP; w += 4) {
-        const int which = w >= NP, pc = which ? w - NP : w;
+    for (int w = int(threadIdx.x >> 6); w < 2 * NC; w += 4) {
+        const int which = w >= NC, c = which ? w - NC : w;
         const uint8_t *tile = p.pool + p.tile_at(j.page, j.head, which, j.base, TB);
-        const uint4 raw = *reinterpret_cast<const uint4 *>(tile + (pc * 64 + lane) * 16);
-        const uint32_t a[4] = {raw.x, raw.y, raw.z, raw.w};
         if (!which) {
-            constexpr int NB = Q8 ? 2 : 1;
-            const int c = Q8 ? pc : pc >> 1;
+            const int t0 = 8 * (lr >> 2) + (lr & 3);
+            u4_t raw[2];
+            if constexpr (Q8) {
+                raw[0] = *reinterpret_cast<const u4_t *>(tile + (c * 64 + lane) * 16);
+            } else {
 #pragma unroll
-            for (int e = 0; e < NB; ++e) {
-                const int t = 8 * (lr >> 2) + 4 * (Q8 ? e : pc & 1) + (lr & 3), pos = j.base + t;
-                if (pos < j.first || pos >= j.s.ctx) continue;
-                float x[8];
+                for (int b = 0; b < 2; ++b) raw[b] = *reinterpret_cast<const u4_t *>(tile + ((2 * c + b) * 64 + lane) * 16);
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int pos = j.base + t0 + 4 * b;
+                f4_t x[2];
                 if constexpr (Q8) {
-                    const float d = h2f(*reinterpret_cast<const uint16_t *>(tile + kv_scale_byte(HD, t, c)));
+                    const float d = h2f(*reinterpret_cast<const uint16_t *>(tile + kv_scale_byte(HD, t0 + 4 * b, c)));
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) x[n] = float(int(a[2 * e + (n >> 2)] << (24 - 8 * (n & 3))) >> 24) * d;
+                    for (int n = 0; n < 8; ++n) x[n >> 2][n & 3] = i8_of(raw[0][2 * b + (n >> 2)], n & 3) * d;
                 } else {
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) x[n] = h2f(a[n >> 1] >> (16 * (n & 1)));
+                    for (int n = 0; n < 8; ++n) x[n >> 2][n & 3] = h2f(raw[b][n >> 1] >> (16 * (n & 1)));
                 }
-                float4 *dst = reinterpret_cast<float4 *>(k + size_t(j.s.r0 + pos - j.first) * ldk +
-                                                         size_t(j.head) * HD + 32 * c + 8 * g);
-                dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-                dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+                trade(x[0], x[1]);
+                if (pos < j.first || pos >= j.s.ctx) continue;
+                f4_t *dst = reinterpret_cast<f4_t *>(k + size_t(j.s.r0 + pos - j.first) * ldk + size_t(j.head) * HD +
+                                                     32 * c) + chunk_of(g);
+                __builtin_nontemporal_store(x[0], dst);
+                __builtin_nontemporal_store(x[1], dst + 4);
             }
         } else {
-            constexpr int NU = Q8 ? 2 : 1;
-            uint4 draw = make_uint4(0, 0, 0, 0);
-            if constexpr (Q8) draw = *reinterpret_cast<const uint4 *>(tile + kv_scale_byte(HD, 8 * g, pc));
-            const uint32_t dd[4] = {draw.x, draw.y, draw.z, draw.w};
+            u4_t raw[2], dd = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if constexpr (Q8) {
+                    const u2_t q = *reinterpret_cast<const u2_t *>(tile + (c * 64 + g * 16 + (2 * lr & 15) + e) * 16 +
+                                                                   8 * (lr >> 3));
+                    raw[e] = u4_t{q[0], q[1], 0u, 0u};
+                } else {
+                    raw[e] = *reinterpret_cast<const u4_t *>(tile + ((2 * c + (lr >> 3)) * 64 + g * 16 + (2 * lr & 15) + e) * 16);
+                }
+            }
+            if constexpr (Q8) dd = *reinterpret_cast<const u4_t *>(tile + kv_scale_byte(HD, 8 * g, c));
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const int pos = j.base + 8 * g + n;
-                if (pos < j.first || pos >= j.s.ctx) continue;
-                float *dst = v + size_t(j.s.r0 + pos - j.first) * ldv + size_t(j.head) * HD + 16 * NU * pc + lr;
+                f2_t x;
                 if constexpr (Q8) {
                     const float d = h2f(dd[n >> 1] >> (16 * (n & 1)));
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        dst[16 * u] = float(int(a[2 * u + (n >> 2)] << (24 - 8 * (n & 3))) >> 24) * d;
+                    x = f2_t{i8_of(raw[0][n >> 2], n & 3) * d, i8_of(raw[1][n >> 2], n & 3) * d};
                 } else {
-                    dst[0] = h2f(a[n >> 1] >> (16 * (n & 1)));
+                    x = f2_t{h2f(raw[0][n >> 1] >> (16 * (n & 1))), h2f(raw[1][n >> 1] >> (16 * (n & 1)))};
                 }
+                if (pos < j.first || pos >= j.s.ctx) continue;
+                __builtin_nontemporal_store(x, reinterpret_cast<f2_t *>(v + size_t(j.s.r0 + pos - j.first) * ldv +
+                                                                        size_t(j.head) * HD + 32 * c + 2 * lr));
             }
         }
     }
