@@ -731,8 +731,12 @@ struct Plan {
     int limit;               // most rows to a K/V head of a sequence of the first launch
 };
 constexpr int kFewSplits = 8;
-constexpr int kFewJobs = 2048, kManyJobs = 1536;  // workgroups of a launch, about
-constexpr int kManyRows = 64;  // of a workgroup of the second launch: RG 2, and QT 2 (hd 256: RG 4, QT 1)
+constexpr int kFewJobs = 2048;  // workgroups of the first launch, about
+// The second launch's shape by head size.
+constexpr int many_qt(int hd) { return hd <= 128 ? 2 : 1; }
+constexpr int many_rg(int) { return 2; }
+constexpr int many_tg(int) { return 2; }
+constexpr int many_rows(int hd) { return many_qt(hd) * many_rg(hd) * kRows; }
 Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx, bool uniform) {
     Plan c;
     const long long most = (long long)max_new * (heads / p.heads);
@@ -741,12 +745,17 @@ Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, in
     const int by_block = kRows / (hd / 32);
     c.blocks = q8 && hd > 32 && (c.many || most <= by_block);
     c.limit = c.blocks ? by_block : kRows;
-    c.tiles = int((most + kManyRows - 1) / kManyRows);
-    // workgroups of the launch that has the most of the work: one for every 64 rows, at least one a sequence
-    const long long of_rows = ((long long)rows * (heads / p.heads) + kManyRows - 1) / kManyRows;
+    const int wg = many_rows(hd);
+    c.tiles = int((most + wg - 1) / wg);
+    // workgroups of the launch that has the most of the work: one for every row tile of it
+    const long long of_rows = ((long long)rows * (heads / p.heads) + wg - 1) / wg;
     const long long jobs = (long long)p.heads * (c.many ? of_rows : p.seqs);
-    long long s = (c.many ? kManyJobs : kFewJobs) / jobs;
-    s = s < max_ctx / (c.many ? 512 : 256) ? s : max_ctx / (c.many ? 512 : 256);
+    // what the GPU holds at once of the second launch: once that for sequences of one length, three times
+    // for ragged ones, whose longest would otherwise run alone at the end
+    const int held = 256 * (hd <= 64 ? 3 : hd <= 128 ? 2 : 1);
+    const bool ragged = (long long)rows * 2 < (long long)p.seqs * max_new;
+    long long s = (!c.many ? kFewJobs : ragged ? 3 * held : held) / jobs;
+    s = s < max_ctx / 256 ? s : max_ctx / 256;
     c.splits = s < 1 ? 1 : int(s);
     return c;
 }
@@ -771,7 +780,7 @@ hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx
     if (pairs > 0x7fffffffll || many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
     constexpr int kAll = 0x7fffffff;
     if (c.many) {
-        constexpr int QT = HD <= 128 ? 2 : 1, RG = kManyRows / (QT * kRows), TG = HD <= 128 ? 2 : 1;
+        constexpr int QT = many_qt(HD), RG = many_rg(HD), TG = many_tg(HD);
         hipLaunchKernelGGL((k_attn<HD, Q8, QT, RG, TG, false>), dim3(unsigned(many)), dim3(64 * RG * TG), 0, st, p, a, r, group,
                            c.tiles, c.splits, c.few ? c.limit : 0, kAll);
     }
