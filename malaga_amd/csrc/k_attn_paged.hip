@@ -464,32 +464,43 @@ __device__ __forceinline__ void put_row(const KvAttn &a, const Work &w, int spli
     }
 }
 
+// Many rows to a K/V head: two groups of many_qt tiles by two waves each.
+constexpr int many_qt(int hd) { return hd <= 128 ? 2 : 1; }
+constexpr int many_rows(int hd) { return 2 * many_qt(hd) * kRows; }
+
 // RG groups of QT tiles of rows, by TG waves each that take every TG-th tile of tokens. Every wave
 // reads its tiles straight into the registers that the matrix products take them from: K of the next
 // tile is asked for once this one's is used, V likewise, so that one of them is always on its way.
 // Waves of other rows read the same lines at about the same time, out of L1 and L2 (a stage through
 // LDS that eight waves shared measured slower: 298 to 376 us against the 4001-token chunk's figure
 // below, for its barriers and because a stage is worked on in less time than the next takes to come).
-// SKIP: sequences of up to that many rows are another launch's; LIMIT: and those of more.
+// Sequences of up to `skip` rows, or more than `limit`, are another shape's.
 template <int HD, bool Q8, int QT, int RG, int TG, bool BLOCKS>
 struct Shape {
-    static constexpr int NC = BLOCKS ? HD / 32 : 1;  // columns of a row
-    static constexpr int kRowsWg = RG * QT * kRows / NC;
+    static constexpr int NC = BLOCKS ? HD / 32 : 1, NU = HD / 16;  // columns of a row
+    static constexpr int kRowsWg = RG * QT * kRows / NC, kThreads = 64 * RG * TG;
     // waves of a SIMD: what the registers of a wave leave room for
     static constexpr int kWavesSimd =
         QT == 1 ? (HD <= 64 ? 4 : HD <= 128 ? (Q8 ? 3 : 2) : 1) : HD <= 64 && QT == 2 ? 3 : 2;
+    // few rows: a K/V head's tiles are read by one workgroup alone, and not again soon
+    static constexpr bool kOnce = RG == 1;
+    struct Lds {
+        f4_t o[TG][RG][QT][NU][64];
+        float m[TG][RG][QT][kRows], l[TG][RG][QT][kRows];
+    };
 };
 
+// Workgroup b of a launch of this shape.
 template <int HD, bool Q8, int QT, int RG, int TG, bool BLOCKS>
-__global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::kWavesSimd)) void k_attn(
-    KvPool pool, KvAttn a, KvRows r, int group, int row_tiles, int splits, int skip, int limit) {
+__device__ __forceinline__ void attn(const KvPool &pool, const KvAttn &a, const KvRows &r, int group, int row_tiles,
+                                     int splits, int skip, int limit, uint32_t b, void *lds) {
     typedef Shape<HD, Q8, QT, RG, TG, BLOCKS> S;
     static_assert(!BLOCKS || (Q8 && QT == 1 && RG == 1), "blocks as columns: one tile of few rows");
     constexpr int TB = kv_tile_bytes(Q8, HD), NU = HD / 16;
-    __shared__ float sm[TG][RG][QT][kRows], sl[TG][RG][QT][kRows];
-    __shared__ f4_t so[TG][RG][QT][NU][64];
+    auto &so = static_cast<typename S::Lds *>(lds)->o;
+    auto &sm = static_cast<typename S::Lds *>(lds)->m;
+    auto &sl = static_cast<typename S::Lds *>(lds)->l;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = w % RG, tg = w / RG;
-    uint32_t b = blockIdx.x;
     Work job;
     job.group = group;
     job.split = int(b % uint32_t(splits));
@@ -538,7 +549,7 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
     int kt = job.split * per + tg;
     bool odd = false;
     uint32_t page = page_of(kt), next = page_of(kt + TG);
-    constexpr bool kOnce = TG == kWaves;
+    constexpr bool kOnce = S::kOnce;
     const uint8_t *at = tile_of(page, kt);
     kr.template load<kOnce>(at, lane);
     vr.template load<kOnce>(at + to_v, lane);
@@ -611,6 +622,40 @@ __global__ __launch_bounds__(64 * RG * TG, (Shape<HD, Q8, QT, RG, TG, BLOCKS>::k
             put_row<HD>(a, job, splits, row, u, lane, o, m, l);
         }
     }
+}
+
+// The launches: few rows, many rows, and both at once (the first `few` workgroups are the few rows'),
+// where the few rows' reads run beside the many rows' arithmetic.
+template <int HD, bool Q8, bool BLOCKS>
+using FewShape = Shape<HD, Q8, 1, 1, kWaves, BLOCKS>;
+template <int HD, bool Q8>
+using ManyShape = Shape<HD, Q8, many_qt(HD), 2, 2, false>;
+
+template <int HD, bool Q8, bool BLOCKS>
+__global__ __launch_bounds__(64 * kWaves, (FewShape<HD, Q8, BLOCKS>::kWavesSimd)) void k_attn_few(
+    KvPool pool, KvAttn a, KvRows r, int group, int splits, int limit) {
+    __shared__ typename FewShape<HD, Q8, BLOCKS>::Lds lds;
+    attn<HD, Q8, 1, 1, kWaves, BLOCKS>(pool, a, r, group, 1, splits, 0, limit, blockIdx.x, &lds);
+}
+template <int HD, bool Q8>
+__global__ __launch_bounds__(64 * kWaves, (ManyShape<HD, Q8>::kWavesSimd)) void k_attn_many(
+    KvPool pool, KvAttn a, KvRows r, int group, int row_tiles, int splits) {
+    __shared__ typename ManyShape<HD, Q8>::Lds lds;
+    attn<HD, Q8, many_qt(HD), 2, 2, false>(pool, a, r, group, row_tiles, splits, 0, 0x7fffffff, blockIdx.x, &lds);
+}
+template <int HD, bool Q8>
+__global__ __launch_bounds__(64 * kWaves, (ManyShape<HD, Q8>::kWavesSimd)) void k_attn_both(
+    KvPool pool, KvAttn a, KvRows r, int group, int row_tiles, int splits, int limit, uint32_t few) {
+    constexpr bool BLOCKS = Q8 && HD > 32;
+    __shared__ union {
+        typename FewShape<HD, Q8, BLOCKS>::Lds few;
+        typename ManyShape<HD, Q8>::Lds many;
+    } lds;
+    if (blockIdx.x < few)
+        attn<HD, Q8, 1, 1, kWaves, BLOCKS>(pool, a, r, group, 1, splits, 0, limit, blockIdx.x, &lds);
+    else
+        attn<HD, Q8, many_qt(HD), 2, 2, false>(pool, a, r, group, row_tiles, splits, limit, 0x7fffffff,
+                                               blockIdx.x - few, &lds);
 }
 
 // Whether some sequence has the row, for the 64 / LANES rows of a wave at once (each the same in its
@@ -722,21 +767,16 @@ __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows
     }
 }
 
-// How a call is cut: sequences of up to kRows rows to a K/V head (group * rows) are one launch's, the
-// others another's, and the tokens of both go into `splits` shares: as many as fill the GPU's compute
-// units (few rows: twice, so that sequences of different lengths even out), none under 256 tokens.
+// How a call is cut: sequences of up to `limit` rows to a K/V head (group * rows) to the few rows' shape,
+// the others to the many rows', and the tokens of both into `splits` shares: as many as fill the GPU's
+// compute units (few rows: twice, so that sequences of different lengths even out), none under 256 tokens.
 struct Plan {
-    int splits, tiles;  // shares; row tiles of the second launch
-    bool few, many, blocks;  // blocks: the few rows' columns are blocks (q8_0)
-    int limit;               // most rows to a K/V head of a sequence of the first launch
+    int splits, tiles;        // shares; row tiles of the many rows' shape
+    bool few, many, blocks;   // blocks: the few rows' columns are blocks (q8_0)
+    int limit;
 };
 constexpr int kFewSplits = 8;
 constexpr int kFewJobs = 2048;  // workgroups of the first launch, about
-// The second launch's shape by head size.
-constexpr int many_qt(int hd) { return hd <= 128 ? 2 : 1; }
-constexpr int many_rg(int) { return 2; }
-constexpr int many_tg(int) { return 2; }
-constexpr int many_rows(int hd) { return many_qt(hd) * many_rg(hd) * kRows; }
 Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx, bool uniform) {
     Plan c;
     const long long most = (long long)max_new * (heads / p.heads);
@@ -777,21 +817,21 @@ hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx
     const bool few = c.splits <= kFewSplits;
     const int per = few ? 256 / (HD / 4) : kWaves;  // (row, head)s of a workgroup of the join
     const long long joins = ((long long)r.rows * a.heads + per - 1) / per;
-    if (pairs > 0x7fffffffll || many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
-    constexpr int kAll = 0x7fffffff;
-    if (c.many) {
-        constexpr int QT = many_qt(HD), RG = many_rg(HD), TG = many_tg(HD);
-        hipLaunchKernelGGL((k_attn<HD, Q8, QT, RG, TG, false>), dim3(unsigned(many)), dim3(64 * RG * TG), 0, st, p, a, r, group,
-                           c.tiles, c.splits, c.few ? c.limit : 0, kAll);
-    }
-    if (c.few && !c.blocks)
-        hipLaunchKernelGGL((k_attn<HD, Q8, 1, 1, kWaves, false>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p, a,
-                           r, group, 1, c.splits, 0, c.limit);
-    if constexpr (Q8 && HD > 32) {
-        if (c.few && c.blocks)
-            hipLaunchKernelGGL((k_attn<HD, Q8, 1, 1, kWaves, true>), dim3(unsigned(pairs)), dim3(64 * kWaves), 0, st, p,
-                               a, r, group, 1, c.splits, 0, c.limit);
-    }
+    if (pairs + many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
+    constexpr bool kByBlock = Q8 && HD > 32;
+    const dim3 threads(64 * kWaves);
+    if (c.many && c.few)
+        hipLaunchKernelGGL((k_attn_both<HD, Q8>), dim3(unsigned(pairs + many)), threads, 0, st, p, a, r, group, c.tiles,
+                           c.splits, c.limit, unsigned(pairs));
+    else if (c.many)
+        hipLaunchKernelGGL((k_attn_many<HD, Q8>), dim3(unsigned(many)), threads, 0, st, p, a, r, group, c.tiles,
+                           c.splits);
+    else if (c.blocks)
+        hipLaunchKernelGGL((k_attn_few<HD, Q8, kByBlock>), dim3(unsigned(pairs)), threads, 0, st, p, a, r, group,
+                           c.splits, c.limit);
+    else
+        hipLaunchKernelGGL((k_attn_few<HD, Q8, false>), dim3(unsigned(pairs)), threads, 0, st, p, a, r, group, c.splits,
+                           c.limit);
     if (c.splits > 1 && few)
         hipLaunchKernelGGL((k_attn_join_few<HD>), dim3(unsigned(joins)), dim3(256), 0, st, p, a, r, c.splits);
     if (c.splits > 1 && !few)
