@@ -481,7 +481,7 @@ struct Shape {
     static constexpr int kRowsWg = RG * QT * kRows / NC, kThreads = 64 * RG * TG;
     // waves of a SIMD: what the registers of a wave leave room for
     static constexpr int kWavesSimd =
-        QT == 1 ? (HD <= 64 ? 4 : HD <= 128 ? (Q8 ? 3 : 2) : 1) : HD <= 64 && QT == 2 ? 3 : 2;
+        QT == 1 ? (HD <= 64 ? 4 : HD <= 128 ? (BLOCKS ? 3 : 2) : 1) : HD <= 64 && QT == 2 ? 3 : 2;
     // few rows: a K/V head's tiles are read by one workgroup alone, and not again soon
     static constexpr bool kOnce = RG == 1;
     struct Lds {
@@ -715,20 +715,24 @@ __global__ __launch_bounds__(256) void k_attn_join_few(KvPool pool, KvAttn a, Kv
     *reinterpret_cast<f4_t *>(a.out + qrow * a.ldo + size_t(head) * HD + 4 * lane) = y;
 }
 
-// The same for many: a wave to a (row, head). Lane k weighs split k, all of their m and l read at once;
-// then the outs, 16 bytes a lane, as many splits at a time as a wave has lanes for.
+// The same for many: a workgroup to a (row, head), each wave a quarter of the splits. Lane k weighs the
+// quarter's split k, all of their m and l read at once; then the outs, 16 bytes a lane, as many splits at
+// a time as a wave has lanes for. The waves meet in LDS.
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows r, int splits) {
     constexpr int LANES = HD / 4, AT = 64 / LANES, PART = HD + kPartHead;  // lanes of an out; outs at a time
-    const int lane = threadIdx.x & 63;
-    const size_t job = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6), qrow = job / size_t(a.heads);
+    __shared__ float sm[kWaves], sl[kWaves];
+    __shared__ f4_t so[kWaves][LANES];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const size_t job = blockIdx.x, qrow = job / size_t(a.heads);
     const int head = int(job % size_t(a.heads));
-    if (!is_a_row<64>(pool, r, qrow) || qrow >= size_t(r.rows)) return;
-    const float *part = a.scratch + (qrow * size_t(a.heads) + size_t(head)) * size_t(splits) * size_t(PART);
+    if (!is_a_row<64>(pool, r, qrow) || qrow >= size_t(r.rows)) return;  // the workgroup's alike
+    const float *part = a.scratch + job * size_t(splits) * size_t(PART);
+    const int quarter = (splits + kWaves - 1) / kWaves, first = w * quarter, end = min(splits, first + quarter);
     float m = -INFINITY, l = 0.f;
     f4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < splits; k0 += 64) {
-        const int n = min(64, splits - k0);
+    for (int k0 = first; k0 < end; k0 += 64) {
+        const int n = min(64, end - k0);
         const float *pk = part + size_t(k0) * PART;
         float mk = -INFINITY, lk = 0.f;
         if (lane < n) {
@@ -751,7 +755,8 @@ __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows
                 fk[j] = __shfl(f, z & 63);
                 const float lz = __shfl(lk, z & 63);  // all lanes
                 x[j] = f4_t{0.f, 0.f, 0.f, 0.f};
-                if (z < last && lz != 0.f) x[j] = *reinterpret_cast<const f4_t *>(pk + size_t(z) * PART + kPartHead + 4 * (lane % LANES));
+                if (z < last && lz != 0.f)
+                    x[j] = *reinterpret_cast<const f4_t *>(pk + size_t(z) * PART + kPartHead + 4 * (lane % LANES));
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) o += x[j] * fk[j];
@@ -761,22 +766,35 @@ __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows
     for (int d = LANES; d < 64; d *= 2)
 #pragma unroll
         for (int n = 0; n < 4; ++n) o[n] += __shfl_xor(o[n], d);
-    if (lane < LANES) {
-        const f4_t y = l == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : o / l;
-        *reinterpret_cast<f4_t *>(a.out + qrow * a.ldo + size_t(head) * HD + 4 * lane) = y;
+    if (lane < LANES) so[w][lane] = o;
+    if (lane == 0) {
+        sm[w] = m;
+        sl[w] = l;
     }
+    __syncthreads();
+    if (w > 0 || lane >= LANES) return;
+    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    l = 0.f;
+    o = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        if (sl[k] == 0.f) continue;
+        const float f = sm[k] == m ? 1.f : __builtin_amdgcn_exp2f(sm[k] - m);
+        l += f * sl[k];
+        o += so[k][lane] * f;
+    }
+    const f4_t y = l == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : o / l;
+    *reinterpret_cast<f4_t *>(a.out + qrow * a.ldo + size_t(head) * HD + 4 * lane) = y;
 }
 
 // How a call is cut: sequences of up to `limit` rows to a K/V head (group * rows) to the few rows' shape,
-// the others to the many rows', and the tokens of both into `splits` shares: as many as fill the GPU's
-// compute units (few rows: twice, so that sequences of different lengths even out), none under 256 tokens.
+// the others to the many rows', and the tokens of both into `splits` shares, none under 256 tokens.
 struct Plan {
     int splits, tiles;        // shares; row tiles of the many rows' shape
     bool few, many, blocks;   // blocks: the few rows' columns are blocks (q8_0)
     int limit;
 };
 constexpr int kFewSplits = 8;
-constexpr int kFewJobs = 2048;  // workgroups of the first launch, about
 Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx, bool uniform) {
     Plan c;
     const long long most = (long long)max_new * (heads / p.heads);
@@ -787,14 +805,19 @@ Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, in
     c.limit = c.blocks ? by_block : kRows;
     const int wg = many_rows(hd);
     c.tiles = int((most + wg - 1) / wg);
-    // workgroups of the launch that has the most of the work: one for every row tile of it
+    // Workgroups without splits, of the shape that has the most of the work, and how many the GPU holds.
     const long long of_rows = ((long long)rows * (heads / p.heads) + wg - 1) / wg;
     const long long jobs = (long long)p.heads * (c.many ? of_rows : p.seqs);
-    // what the GPU holds at once of the second launch: once that for sequences of one length, three times
-    // for ragged ones, whose longest would otherwise run alone at the end
-    const int held = 256 * (hd <= 64 ? 3 : hd <= 128 ? 2 : 1);
+    const int held = 256 * (c.many ? (hd <= 64 ? 3 : hd <= 128 ? 2 : 1) : hd <= 64 ? 4 : hd > 128 ? 1 : c.blocks ? 3 : 2);
+    // Many rows: as many as it holds; twice that for ragged sequences, whose longest would run alone at
+    // the end otherwise (q8_0 mix of single tokens and chunks of 33 .. 517 rows: 90 us so, 100 us with three
+    // times, 113 us unsplit; a chunk of 4001 rows: 208 us unsplit, 231 us in two).
+    // Few rows: half as many again where the heads are too few to fill it (3 contexts of 60000 .. 100002
+    // tokens, 8 heads: 150 us, 156 us with twice, 159 us with three times as many); else two shares for
+    // up to 1024 heads, against ragged lengths (64 sequences of 91 .. 2301 tokens, 16 heads: 70 us, 73 us unsplit).
     const bool ragged = (long long)rows * 2 < (long long)p.seqs * max_new;
-    long long s = (!c.many ? kFewJobs : ragged ? 3 * held : held) / jobs;
+    const long long most_jobs = c.many ? (ragged ? 2 : 1) * held : jobs < held ? held + held / 2 : 2048;
+    long long s = most_jobs / jobs;
     s = s < max_ctx / 256 ? s : max_ctx / 256;
     c.splits = s < 1 ? 1 : int(s);
     return c;
@@ -815,7 +838,7 @@ hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx
     const Plan c = plan(p, Q8, HD, a.heads, r.rows, r.max_new, max_ctx, !r.row_off);
     const long long pairs = (long long)p.seqs * p.heads * c.splits, many = pairs * c.tiles;
     const bool few = c.splits <= kFewSplits;
-    const int per = few ? 256 / (HD / 4) : kWaves;  // (row, head)s of a workgroup of the join
+    const int per = few ? 256 / (HD / 4) : 1;  // (row, head)s of a workgroup of the join
     const long long joins = ((long long)r.rows * a.heads + per - 1) / per;
     if (pairs + many > 0x7fffffffll || joins > 0x7fffffffll) return hipErrorInvalidValue;
     constexpr bool kByBlock = Q8 && HD > 32;
