@@ -68,13 +68,14 @@ __device__ __forceinline__ Q8Scale q8_scale(float amax) {
 // below 0.5 added with x's sign rounds to the next integer exactly where the half does (at y + 0.5 - 2^-25
 // a tie goes to the even number, which is the integer), and leaves all that is below the half below it.
 // inf times inv = 0 is NaN, which converts to 0.
-__device__ __forceinline__ uint32_t q8_four(float a, float b, float c, float d, float inv) {
-    auto one = [&](float x) __attribute__((always_inline)) {
-        const float y = __fmul_rn(x, inv);
-        return uint32_t(int(__fadd_rn(y, copysignf(0x1.fffffep-2f, y))));
+__device__ __forceinline__ uint32_t q8_four(float a, float b, float c, float d, float ia, float ib, float ic, float id) {
+    auto one = [](float x, float inv) __attribute__((always_inline)) {
+        float y = x * inv;
+        asm("" : "+v"(y));  // rounded here: the compiler would make one operation of the product and the sum
+        return uint32_t(int(y + copysignf(0x1.fffffep-2f, y)));
     };
-    const uint32_t lo = __builtin_amdgcn_perm(one(b), one(a), 0x0c0c0400u);
-    const uint32_t hi = __builtin_amdgcn_perm(one(d), one(c), 0x04000c0cu);
+    const uint32_t lo = __builtin_amdgcn_perm(one(b, ib), one(a, ia), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(one(d, id), one(c, ic), 0x04000c0cu);
     return lo | hi;
 }
 __device__ __forceinline__ float largest(float m, float x) {  // inf for a value that is not finite
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvPool p, const float *k, size
                     const Q8Scale sc = q8_scale(amax);
                     u2_t q;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) q[h] = q8_four(x[b][h][0], x[b][h][1], x[b][h][2], x[b][h][3], sc.inv);
+                    for (int h = 0; h < 2; ++h) q[h] = q8_four(x[b][h][0], x[b][h][1], x[b][h][2], x[b][h][3], sc.inv, sc.inv, sc.inv, sc.inv);
                     if (in[b]) {
                         *reinterpret_cast<u2_t *>(tile + (c * 64 + lane) * 16 + 8 * b) = q;
                         if (g == 0) *reinterpret_cast<uint16_t *>(tile + kv_scale_byte(HD, t0 + 4 * b, c)) = uint16_t(sc.d);
@@ -200,10 +201,8 @@ __global__ __launch_bounds__(256) void k_kv_write(KvPool p, const float *k, size
                     u2_t q;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float y[4];
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) y[n] = __fmul_rn(x[4 * h + n][e], inv[4 * h + n]);
-                        q[h] = q8_four(y[0], y[1], y[2], y[3], 1.f);
+                        const f4_t y = {x[4 * h][e], x[4 * h + 1][e], x[4 * h + 2][e], x[4 * h + 3][e]};
+                        q[h] = q8_four(y[0], y[1], y[2], y[3], inv[4 * h], inv[4 * h + 1], inv[4 * h + 2], inv[4 * h + 3]);
                     }
                     uint8_t *at = tile + (c * 64 + g * 16 + (2 * lr & 15) + e) * 16 + 8 * (lr >> 3);
                     if (all) {

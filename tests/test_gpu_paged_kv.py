@@ -203,6 +203,26 @@ def test_values_that_are_not_finite_and_the_edges_of_the_formats():
     assert (got[3, 0, :32] == 0).all() and not np.isfinite(got[3, 0, 32])  # a scale beyond f16
 
 
+def test_quotients_next_to_a_half_round_as_the_codec_rounds_them():
+    """q8_0 values whose quotient by the scale is a half of a whole number or a few units in the last place
+    beside it, for many scales: a product and a sum taken in one rounding would move some of them."""
+    rng = np.random.default_rng(17)
+    n, heads, hd = 512, 8, 64
+    amax = rng.uniform(0.5, 4.0, (n, heads, 2, 1)).astype(np.float32)
+    d = (amax / np.float32(127)).astype(np.float32)
+    half = rng.integers(0, 126, (n, heads, 2, 32)).astype(np.float32) + np.float32(0.5)
+    x = (half * d).astype(np.float32)
+    x = (x.view(np.int32) + rng.integers(-2, 3, x.shape)).astype(np.int32).view(np.float32)
+    x *= rng.choice([-1.0, 1.0], x.shape).astype(np.float32)
+    x[..., 5:6] = amax
+    x = x.reshape(n, heads, hd)
+    c = Cache(Q8_0, heads, hd, 64, 1, n // 64)
+    put(c, dev(x), dev(x[::-1].copy()), [n], [n])
+    k, v = torch.zeros(n, heads, hd, device="cuda"), torch.zeros(n, heads, hd, device="cuda")
+    get(c, k, v, [n], [n])
+    assert np.array_equal(k.cpu().numpy(), c.stored(x)) and np.array_equal(v.cpu().numpy(), c.stored(x[::-1].copy()))
+
+
 ATTEND = [  # kind, hd, K/V heads, group, page
     (F16, 64, 2, 1, 64), (Q8_0, 64, 2, 1, 64), (F16, 32, 1, 3, 32), (Q8_0, 32, 2, 2, 256), (F16, 128, 1, 5, 128),
     (Q8_0, 128, 2, 1, 32), (F16, 256, 1, 2, 64), (Q8_0, 256, 1, 7, 32), (F16, 64, 1, 16, 32), (Q8_0, 64, 1, 24, 64),
