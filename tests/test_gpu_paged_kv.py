@@ -334,6 +334,85 @@ def test_sizes_of_the_operands(kind):
         assert (np.abs(got - want) <= err).all(), (vs, qs)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.125, 0.125])
+@pytest.mark.parametrize("n", [2, 40])
+def test_scales_of_any_sign(n, scale):
+    """Scale 0 weighs all that a row sees alike; a negative one prefers what a positive one avoids."""
+    for kind in KINDS:
+        cache, held, rng = filled(kind, 1, 64, 32, [(n, 75)], 6)
+        q = rng.normal(0, 1, (n, 2, 64)).astype(np.float32)
+        got = attend(cache, dev(q), [n], [75], scale).cpu().numpy()
+        want, err = reference(q, *held[0], n, 75, scale, True)
+        assert (np.abs(got - want) <= err).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_values_of_zero_before_others(hd, n):
+    """q8_0: long runs of V that is zero, in all blocks or in one, before the first scale that is not."""
+    rng = np.random.default_rng(12)
+    ctx = 700
+    k, v = (rng.normal(0, 1, (ctx, 1, hd)).astype(np.float32) for _ in range(2))
+    v[:400] = 0
+    v[400:600, :, :32] = 0
+    cache = Cache(Q8_0, 1, hd, 64, 1, 11)
+    put(cache, dev(k), dev(v), [ctx], [ctx])
+    q = rng.normal(0, 1, (n, 1, hd)).astype(np.float32)
+    got = attend(cache, dev(q), [n], [ctx], 0.125).cpu().numpy()
+    want, err = reference(q, cache.stored(k), cache.stored(v), n, ctx, 0.125, True)
+    assert (np.abs(got - want) <= err).all()
+
+
+@pytest.mark.parametrize("hd,heads,seqs,longest", [(32, 2, 150, 2100), (64, 1, 90, 4100), (256, 1, 70, 1500)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_sequences_in_splits(kind, hd, heads, seqs, longest):
+    """More sequences than a wave has lanes, ragged and some without rows, a bad one among them, their tokens
+    split: the join finds every row's sequence, and no other row."""
+    rng = np.random.default_rng(seqs)
+    ctx = rng.integers(1, 60, seqs).tolist()
+    ctx[3], ctx[-1] = longest, longest - 77
+    new = [min(c, int(x)) for c, x in zip(ctx, rng.integers(0, 3, seqs))]
+    new[3], new[-1] = 2, 1
+    cache, held, rng = filled(kind, heads, hd, 64, list(zip(new, ctx)), seqs)
+    q = rng.normal(0, 1, (sum(new) + 3, heads, hd)).astype(np.float32)
+    assert lib.mlg_attn_paged_scratch(C.byref(cache.c), heads, len(q), 2, 0) > 0
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    told = list(ctx)
+    told[5] = 64 * cache.table_len + 1  # more than its table row holds
+    got = attend(cache, dev(q), new, told, 1 / np.sqrt(hd), bad=bad).cpu().numpy()
+    assert bad.item() == 1 and (got[sum(new):] == 7).all()
+    off = rows_of(new)
+    assert (got[off[5]:off[6]] == 0).all()
+    for i in (0, 2, 3, 4, 6, 63, 64, 65, seqs - 2, seqs - 1):
+        want, err = reference(q[off[i]:off[i + 1]], *held[i], new[i], ctx[i], 1 / np.sqrt(hd), True)
+        assert (np.abs(got[off[i]:off[i + 1]] - want) <= err).all(), i
+
+
+@pytest.mark.parametrize("n", [1, 50])
+def test_out_in_the_place_of_q(n):
+    cache, held, rng = filled(F16, 2, 64, 32, [(n, 90), (n, 64)], 15)
+    q = dev(rng.normal(0, 1, (2 * n, 4, 64)).astype(np.float32))
+    want = attend(cache, q, [n, n], [90, 64], 0.125)
+    attend(cache, q, [n, n], [90, 64], 0.125, out=q)
+    assert torch.equal(q, want)
+
+
+def test_calls_on_two_streams_at_once():
+    """Two caches written and attended on two streams without a wait between them: each as if alone."""
+    made = [filled(kind, 2, 64, 64, [(1, 3000), (1, 40)], 20 + kind) for kind in KINDS]
+    qs = [dev(rng.normal(0, 1, (2, 2, 64)).astype(np.float32)) for _, _, rng in made]
+    want = [attend(c, q, [1, 1], [3000, 40], 0.125) for (c, _, _), q in zip(made, qs)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in made], []
+    for _ in range(20):
+        for st, (c, _, _), q in zip(streams, made, qs):
+            with torch.cuda.stream(st):
+                got.append(attend(c, q, [1, 1], [3000, 40], 0.125, sync=False))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g, want[i % 2])
+
+
 def test_a_query_that_is_not_finite_spoils_its_own_row_alone():
     cache, held, rng = filled(F16, 1, 64, 32, [(4, 50)], 3)
     q = rng.normal(0, 1, (4, 1, 64)).astype(np.float32)

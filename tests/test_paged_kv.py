@@ -151,6 +151,19 @@ def test_refusals_of_the_attention():
 
 
 @pytest.mark.parametrize("call", [write, read, attend])
+def test_sizes_beyond_the_kernels_indexes(call):
+    """Pages of 2^32 bytes, and launches of more workgroups or rows than a grid or an int has."""
+    big = cache(heads=1 << 18, head_size=128, page=256)
+    assert call(C.byref(big), ld=1 << 27, ldv=1 << 27, **(dict(heads=1 << 18) if call is attend else {})) == _lib.ERR_INVALID
+    wide = cache(seqs=1 << 30, heads=8)
+    assert call(C.byref(wide), ld=1024, **(dict(heads=8, scratch=16, size=1 << 62) if call is attend else {})) == \
+        _lib.ERR_INVALID
+    if call is attend:
+        assert attend(C.byref(cache(seqs=1, heads=1)), ld=1 << 20, ldv=1 << 20, heads=1 << 14, max_new=1 << 20,
+                      scratch=16, size=1 << 62) == _lib.ERR_INVALID
+
+
+@pytest.mark.parametrize("call", [write, read, attend])
 def test_nothing_to_do_is_ok(call):
     """No sequences, or no rows: no launch, so no device either."""
     assert call(C.byref(cache(seqs=0))) == _lib.OK
